@@ -125,7 +125,9 @@ int32_t tmx_sm_count(void);
 /* Set an integer option on a loaded kernel.  Known options: "causal" (attention
  * kernels: mask key j > query i), "path" (0 = automatic, 1 = force the generic
  * SIMT kernel, 2 = require a tensor-core kernel - tcgen05 for 16-bit elements,
- * 3xTF32 for fp32 - and fail if the shape is not eligible).  0 / -1. */
+ * 3xTF32 for fp32 - and fail if the shape is not eligible), "activation" (feed-forward kernels:
+ * 0 none, 1 relu, 2 gelu with erf, 3 gelu with tanh, 4 silu, 5 sigmoid), "layer_norm" (norm kernels:
+ * 1 layer norm, 0 root-mean-square norm).  0 / -1. */
 int32_t tmx_kernel_set_option(int64_t kernel, const char *name, int64_t value);
 /* Which implementation the most recent launch of `kernel` used:
  * 0 none yet, 1 generic SIMT, 2 tcgen05.  -1 on a bad handle. */
@@ -142,6 +144,17 @@ int32_t tmx_launch_timed(int64_t kernel, int64_t grid_x, int64_t grid_y, int64_t
                          int64_t threads_per_threadgroup, const int32_t *kinds,
                          const int64_t *values, int32_t arg_count, int32_t repeats,
                          float *elapsed_ms);
+/* Enqueue a feed-forward kernel (linear_kernel and the others listed at the end of this file) on a
+ * CUDA stream of the caller's and return.  Kinds 0...3 as in tm_launch; kind 4 is a device address in
+ * values[i] with lengths[i] bytes behind it (memory of the library's device, of any allocator; the
+ * address of an operand without elements may be 0).  The call is ordered by that stream alone and may be captured into a
+ * graph: the kernels keep nothing between calls, and what scratch memory they need is allocated and
+ * freed in stream order.  A buffer handle (kind 0) is ordered by the library's stream and accepted only
+ * there (stream == tmx_stream_handle()).  The calling thread's current device stays as it was.
+ * A bounded wait that gives up inside the kernel is reported by the next synchronising tm_* call. */
+int32_t tmx_launch_on(int64_t kernel, void *stream, int64_t grid_x, int64_t grid_y, int64_t grid_z,
+                      int64_t threads_per_threadgroup, const int32_t *kinds, const int64_t *values,
+                      const int64_t *lengths, int32_t arg_count);
 /* Wait for everything enqueued on the library's stream; surfaces device-side
  * status words (bounded waits that gave up) as -1. */
 int32_t tmx_synchronize(void);
@@ -279,6 +292,42 @@ int64_t tmx_debug_attention_schedule(int32_t kind, int32_t bh, int32_t rows, int
                                      int64_t *load_out);
 /* Set the device status word from the host, as a kernel whose wait gave up would. */
 int32_t tmx_debug_inject_status(int32_t code, int32_t where, int32_t block, int32_t extra);
+
+/* ---- the feed-forward kernels (no counterpart in the reference) -------------
+ *
+ * The other half of a transformer layer, loaded and launched like the kernels above (tm_emit_msl on
+ * IR that names one of them, tm_load_kernel, tm_launch / tmx_launch_async / tmx_launch_timed, or
+ * tmx_launch_on).  Element type f32, f16 or bf16, one for all operands; arguments are matched by
+ * name, those in brackets may be left out of the signature, strides default to dense row-major.
+ * All sums are formed in fp32 and every output is rounded once, except where noted.  An output may
+ * not overlap another operand, but out may be residual itself, dz (dgate, dup) an input of the same
+ * shape, sum or normed may be residual or block, dresidual may be dsum or dnormed, and dblock may be
+ * dsum, dnormed or block.
+ *
+ *   linear_kernel(x, w, [bias], [residual], out, [pre], M, N, K, [stride_xm, stride_xk, stride_wk,
+ *                 stride_wn, stride_om, stride_rm, stride_pm])
+ *       pre = x w + bias, out = act(pre) + residual (act takes the unrounded value)
+ *   gated_linear_kernel(x, w_gate, w_up, out, [pre_gate], [pre_up], M, N, K, [strides as above])
+ *       pre_gate = x w_gate, pre_up = x w_up, out = act(pre_gate) * pre_up
+ *   linear_sum_kernel(x, w, x2, w2, out, M, N, K, [strides])       out = x w + x2 w2
+ *   linear_pair_kernel(x, w, x2, w2, out, out2, M, N, K, [strides])  out = x w, out2 = x2 w2
+ *   activation_bwd_kernel(dout, [pre], [dz], [dbias], M, N, [stride_dout, stride_pre, stride_dz])
+ *       dz = dout act'(pre), dbias[n] = sum over m of the unrounded dz
+ *   gated_activation_bwd_kernel(dout, pre_gate, pre_up, dgate, dup, M, N, [strides as above])
+ *       dgate = dout pre_up act'(pre_gate), dup = dout act(pre_gate)
+ *   residual_norm_kernel(residual, [block], weight, [bias], [gate], [post_weight], [sum], normed,
+ *                        [stats], scale, eps, M, D, [stride_row])
+ *       t = post_weight ? N(block) post_weight : block;  sum = scale residual + gate t;
+ *       normed = N(sum) weight + bias, N being the root-mean-square norm or layer norm ("layer_norm",
+ *       or attribute tm.norm = "layer"); stats[row] = {mean, 1/deviation} of sum, then of block, fp32
+ *   residual_norm_bwd_kernel(dnormed, [dsum], sum, stats, weight, [block], [gate], [post_weight],
+ *                            [dresidual], [dblock], [dweight], [dbias], [dgate], [dpost_weight], scale,
+ *                            M, D, [stride_row])
+ * The grid has the meaning of the IR's block shape, as for matmul_kernel: rows beyond grid_x * BLOCK_M
+ * (and, for the products and activation gradients, columns beyond grid_y * BLOCK_N) are left as they
+ * are.  Rows of the norms have at most 16384 columns.  Gradients of a linear layer: dx = dz w^T and
+ * dw = x^T dz are linear_kernel launches with transposed strides; of a gated one, dx is
+ * linear_sum_kernel on (dgate, w_gate^T, dup, w_up^T), and dw_gate, dw_up are linear_pair_kernel. */
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,207 @@
+// The element-wise part of the feed-forward backward passes.
+//
+//   activation_bwd_kernel        dz = dout * act'(pre),  dbias[n] = sum_m dz[m, n]
+//   gated_activation_bwd_kernel  dgate = dout * up * act'(gate),  dup = dout * act(gate)
+//
+// HBM-bound: every operand is read or written once, in 16-byte packets where the rows allow.  A
+// block is 32 packets wide and 8 rows high and walks down its share of the rows, so a warp's
+// access is 512 contiguous bytes and each thread keeps the column sums of dz (fp32, before dz is
+// rounded) in registers.  The sums of a block are joined in shared memory, those of several row
+// blocks through scratch memory in a second kernel: a fixed order, so that a call always gives the
+// same bits.
+
+#include "ffn_math.cuh"
+
+#include <algorithm>
+#include <mutex>
+
+namespace tmc {
+
+// ---- stream-ordered scratch -------------------------------------------------------------------
+std::string scratch_alloc(const LaunchCtx& ctx, size_t bytes, void** out) {
+  *out = nullptr;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  static std::mutex lock;
+  static cudaMemPool_t pool = nullptr;      // one device per process
+  if (e == cudaSuccess) {
+    std::lock_guard<std::mutex> guard(lock);
+    if (!pool) {
+      cudaMemPoolProps props{};
+      props.allocType = cudaMemAllocationTypePinned;
+      props.handleTypes = cudaMemHandleTypeNone;
+      props.location.type = cudaMemLocationTypeDevice;
+      props.location.id = device;
+      e = cudaMemPoolCreate(&pool, &props);
+      if (e == cudaSuccess) {
+        uint64_t keep = 64ull << 20;         // freed scratch beyond this goes back to the device
+        cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+      }
+    }
+  }
+  if (e == cudaSuccess) e = cudaMallocFromPoolAsync(out, bytes, pool, ctx.stream);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return "could not allocate " + std::to_string(bytes) + " bytes of scratch memory: " + cudaGetErrorString(e);
+  }
+  return std::string();
+}
+void scratch_free(const LaunchCtx& ctx, void* p) {
+  if (p) cudaFreeAsync(p, ctx.stream);
+}
+
+namespace {
+
+using namespace ffn;
+
+constexpr int CX = 32, RY = 8;
+
+template <typename T, int VEC, bool GATED>
+__global__ void __launch_bounds__(CX * RY) activation_bwd_kernel(const ActBwdProblem p, float* __restrict__ partial,
+                                                                 int64_t rows_per_block) {
+  const int tx = threadIdx.x % CX, ty = threadIdx.x / CX;
+  const int64_t col = ((int64_t)blockIdx.x * CX + tx) * VEC;
+  const int64_t first = (int64_t)blockIdx.y * rows_per_block;
+  const int64_t last = min(first + rows_per_block, p.M);
+  float sum[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+  if (col < p.N) {
+    with_act(p.act, [&](auto tag) {
+      constexpr Act act = decltype(tag)::value;
+      constexpr bool precise = sizeof(T) == 4;
+#pragma unroll 2
+      for (int64_t m = first + ty; m < last; m += RY) {
+        float d[VEC];
+        load_vec<T, VEC>((const T*)p.dout + m * p.s_dout + col, d);
+        if constexpr (GATED) {
+          float g[VEC], u[VEC], du[VEC];
+          load_vec<T, VEC>((const T*)p.pre + m * p.s_pre + col, g);
+          load_vec<T, VEC>((const T*)p.up + m * p.s_pre + col, u);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            du[i] = d[i] * act_forward<precise>(act, g[i]);
+            d[i] = d[i] * u[i] * act_derivative<precise>(act, g[i]);
+          }
+          store_vec<T, VEC>((T*)p.dup + m * p.s_dz + col, du);
+        } else if constexpr (act != Act::None) {
+          float z[VEC];
+          load_vec<T, VEC>((const T*)p.pre + m * p.s_pre + col, z);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) d[i] *= act_derivative<precise>(act, z[i]);
+        }
+        if (p.dz) store_vec<T, VEC>((T*)p.dz + m * p.s_dz + col, d);
+        if constexpr (!GATED) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sum[i] += d[i];
+        }
+      }
+    });
+  }
+  if constexpr (!GATED) {
+    if (!p.dbias) return;
+    __shared__ float joined[RY][CX * VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) joined[ty][tx * VEC + i] = sum[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < CX * VEC; c += CX * RY) {
+      float total = 0.f;
+#pragma unroll
+      for (int r = 0; r < RY; ++r) total += joined[r][c];
+      const int64_t n = (int64_t)blockIdx.x * CX * VEC + c;
+      if (n >= p.N) continue;
+      if (partial) partial[(int64_t)blockIdx.y * p.N + n] = total;
+      else ((T*)p.dbias)[n] = from_f32<T>(total);
+    }
+  }
+}
+
+template <typename T, int VEC>
+std::string launch_vec(const ActBwdProblem& p, const LaunchCtx& ctx) {
+  const int64_t gx = (p.N + CX * VEC - 1) / (CX * VEC);
+  // about eight blocks per SM, each with at least 32 rows so that the column sums stay cheap
+  int64_t gy = std::max<int64_t>(1, (int64_t)ctx.sm_count * 8 / gx);
+  gy = std::min(gy, std::max<int64_t>(1, (p.M + 31) / 32));
+  gy = std::min<int64_t>(gy, 65535);
+  const int64_t rows = std::max<int64_t>(1, (p.M + gy - 1) / gy);
+  gy = std::max<int64_t>(1, (p.M + rows - 1) / rows);
+  if (gx > 0x7fffffff) return "too many columns";
+  const dim3 grid((unsigned)gx, (unsigned)gy);
+  if (p.gated) {
+    activation_bwd_kernel<T, VEC, true><<<grid, CX * RY, 0, ctx.stream>>>(p, nullptr, rows);
+    ++*ctx.launches;
+  } else {
+    void* partial = nullptr;
+    if (p.dbias && gy > 1) {
+      std::string err = scratch_alloc(ctx, (size_t)gy * (size_t)p.N * 4, &partial);
+      if (!err.empty()) return err;
+    }
+    activation_bwd_kernel<T, VEC, false><<<grid, CX * RY, 0, ctx.stream>>>(p, (float*)partial, rows);
+    ++*ctx.launches;
+    if (partial) {
+      void* outs[kMaxColumnSums] = {p.dbias};
+      launch_column_sums(p.elt, (const float*)partial, gy, p.N, 1, outs, ctx);
+      scratch_free(ctx, partial);
+    }
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return std::string("activation backward launch failed: ") + cudaGetErrorString(e);
+  return std::string();
+}
+
+template <typename T>
+std::string launch_typed(const ActBwdProblem& p, const LaunchCtx& ctx) {
+  constexpr int VEC = 16 / sizeof(T);
+  uintptr_t bases = (uintptr_t)p.dout | (uintptr_t)p.dz;
+  int64_t strides = p.s_dout | (p.dz ? p.s_dz : 0);
+  if (p.act != Act::None || p.gated) { bases |= (uintptr_t)p.pre; strides |= p.s_pre; }
+  if (p.gated) bases |= (uintptr_t)p.up | (uintptr_t)p.dup;
+  const bool packets = bases % 16 == 0 && strides % VEC == 0 && p.N % VEC == 0;
+  return packets ? launch_vec<T, VEC>(p, ctx) : launch_vec<T, 1>(p, ctx);
+}
+
+// out[n] = sum over `parts` rows of partial[part][n], for up to kMaxColumnSums sets at once.
+struct SumOutputs {
+  void* out[kMaxColumnSums];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ partial, int64_t parts,
+                                                          int64_t N, const SumOutputs outs) {
+  __shared__ float joined[8][33];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t n = (int64_t)blockIdx.x * 32 + tx;
+  const float* base = partial + (int64_t)blockIdx.y * parts * N;
+  float total = 0.f;
+  if (n < N) {
+#pragma unroll 8
+    for (int64_t r = ty; r < parts; r += 8) total += base[r * N + n];
+  }
+  joined[ty][tx] = total;
+  __syncthreads();
+  if (ty == 0 && n < N) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) total += joined[r][tx];
+    ((T*)outs.out[blockIdx.y])[n] = from_f32<T>(total);
+  }
+}
+
+}  // namespace
+
+void launch_column_sums(Elt elt, const float* partial, int64_t parts, int64_t N, int sets, void* const* out,
+                        const LaunchCtx& ctx) {
+  SumOutputs outs{};
+  for (int i = 0; i < sets; ++i) outs.out[i] = out[i];
+  const dim3 grid((unsigned)((N + 31) / 32), (unsigned)sets);
+  if (elt == Elt::F32) column_sums_kernel<float><<<grid, 256, 0, ctx.stream>>>(partial, parts, N, outs);
+  else if (elt == Elt::BF16) column_sums_kernel<__nv_bfloat16><<<grid, 256, 0, ctx.stream>>>(partial, parts, N, outs);
+  else column_sums_kernel<__half><<<grid, 256, 0, ctx.stream>>>(partial, parts, N, outs);
+  ++*ctx.launches;
+}
+
+std::string launch_activation_bwd(const ActBwdProblem& p, const LaunchCtx& ctx) {
+  if (p.elt == Elt::F32) return launch_typed<float>(p, ctx);
+  if (p.elt == Elt::BF16) return launch_typed<__nv_bfloat16>(p, ctx);
+  return launch_typed<__half>(p, ctx);
+}
+
+}  // namespace tmc

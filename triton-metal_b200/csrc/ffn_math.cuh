@@ -1,0 +1,118 @@
+// Element conversions, 16-byte packets, and the activations with their derivatives, in fp32.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "ffn_core.h"
+
+namespace tmc {
+namespace ffn {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// VEC consecutive elements as fp32.  VEC > 1 is one 16-byte access (the address must be aligned to
+// it); the plain loads go through the read-only path with no cache hint.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = to_f32(*p);
+  } else {
+    static_assert(VEC * sizeof(T) == 16, "one packet");
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_f32(e[i]);
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = from_f32<T>(v[0]);
+  } else {
+    static_assert(VEC * sizeof(T) == 16, "one packet");
+    uint4 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<uint4*>(p) = raw;
+  }
+}
+
+// 1 / (1 + exp(-z)): exp overflows to infinity for z < -88 and the quotient is then 0, its limit.
+// __expf and __fdividef err by a few units in the last place of fp32, far below a 16-bit rounding;
+// fp32 operands (PRECISE) take expf and the exact quotient.
+template <bool PRECISE>
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (PRECISE) return 1.f / (1.f + expf(-z));
+  return __fdividef(1.f, 1.f + __expf(-z));
+}
+// z kept inside the range where the derivatives still change (a comparison lets a NaN through):
+// beyond it exp(-z^2/2) and s(1-s) are 0 in fp32 and would meet an overflowed factor.
+__device__ __forceinline__ float bounded(float z) { return z > 100.f ? 100.f : (z < -100.f ? -100.f : z); }
+
+constexpr float kSqrtHalf = 0.70710678118654752440f;
+constexpr float kInvSqrt2Pi = 0.39894228040143267794f;
+constexpr float kTanhA = 0.79788456080286535588f;   // sqrt(2 / pi)
+constexpr float kTanhB = 0.044715f;
+
+// gelu_tanh(z) = z/2 (1 + tanh(a(z + b z^3))) = z sigmoid(2a(z + b z^3)): no cancellation for z < 0.
+template <bool PRECISE>
+__device__ __forceinline__ float act_forward(Act act, float z) {
+  switch (act) {
+    case Act::Relu: return z != z ? z : fmaxf(z, 0.f);          // fmaxf alone would drop a NaN
+    case Act::Gelu: return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+    case Act::GeluTanh: return z * sigmoid<PRECISE>(2.f * kTanhA * (z + kTanhB * z * z * z));
+    case Act::Silu: return z * sigmoid<PRECISE>(z);
+    case Act::Sigmoid: return sigmoid<PRECISE>(z);
+    default: return z;
+  }
+}
+template <bool PRECISE>
+__device__ __forceinline__ float act_derivative(Act act, float z) {
+  z = bounded(z);
+  switch (act) {
+    case Act::Relu: return z != z ? z : (z > 0.f ? 1.f : 0.f);
+    case Act::Gelu: {
+      const float density = kInvSqrt2Pi * (PRECISE ? expf(-0.5f * z * z) : __expf(-0.5f * z * z));
+      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * density;
+    }
+    case Act::GeluTanh: {
+      const float s = sigmoid<PRECISE>(2.f * kTanhA * (z + kTanhB * z * z * z));
+      return s + z * s * (1.f - s) * 2.f * kTanhA * (1.f + 3.f * kTanhB * z * z);
+    }
+    case Act::Silu: {
+      const float s = sigmoid<PRECISE>(z);
+      return s * (1.f + z * (1.f - s));
+    }
+    case Act::Sigmoid: {
+      const float s = sigmoid<PRECISE>(z);
+      return s * (1.f - s);
+    }
+    default: return 1.f;
+  }
+}
+
+// Calls f with the activation as a compile-time constant.
+template <typename F>
+__device__ __forceinline__ void with_act(Act act, F&& f) {
+  switch (act) {
+    case Act::Relu: f(std::integral_constant<Act, Act::Relu>{}); break;
+    case Act::Gelu: f(std::integral_constant<Act, Act::Gelu>{}); break;
+    case Act::GeluTanh: f(std::integral_constant<Act, Act::GeluTanh>{}); break;
+    case Act::Silu: f(std::integral_constant<Act, Act::Silu>{}); break;
+    case Act::Sigmoid: f(std::integral_constant<Act, Act::Sigmoid>{}); break;
+    default: f(std::integral_constant<Act, Act::None>{}); break;
+  }
+}
+
+}  // namespace ffn
+}  // namespace tmc

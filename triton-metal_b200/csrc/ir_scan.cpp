@@ -14,6 +14,7 @@
 
 #include "tm_core.h"
 
+#include <algorithm>
 #include <cctype>
 #include <cstdio>
 #include <cstdlib>
@@ -37,8 +38,23 @@ const char* kernel_entry_name(KernelId id) {
     case KernelId::ScaleBias: return "scale_bias_kernel";
     case KernelId::Softmax: return "softmax_kernel";
     case KernelId::SaeEncode: return "sae_encode_kernel";
+    case KernelId::Linear: return "linear_kernel";
+    case KernelId::GatedLinear: return "gated_linear_kernel";
+    case KernelId::LinearSum: return "linear_sum_kernel";
+    case KernelId::LinearPair: return "linear_pair_kernel";
+    case KernelId::ActBwd: return "activation_bwd_kernel";
+    case KernelId::GatedActBwd: return "gated_activation_bwd_kernel";
+    case KernelId::ResidualNorm: return "residual_norm_kernel";
+    case KernelId::ResidualNormBwd: return "residual_norm_bwd_kernel";
     default: return "?";
   }
+}
+
+static const char* const kActivationNames[] = {"none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid"};
+int activation_from_name(const std::string& name) {
+  for (int i = 0; i < 6; ++i)
+    if (name == kActivationNames[i]) return i;
+  return -1;
 }
 
 namespace {
@@ -94,6 +110,32 @@ Role role_from_name(KernelId id, const std::string& raw) {
         {"c", Role::C}, {"m", Role::M}, {"n", Role::N}, {"k", Role::K},
         {"stride_am", Role::StrideAm}, {"stride_ak", Role::StrideAk}, {"stride_bk", Role::StrideBk},
         {"stride_bn", Role::StrideBn}, {"stride_cm", Role::StrideCm}, {"stride_cn", Role::StrideCn}};
+    auto it = m.find(n);
+    return it == m.end() ? Role::Unknown : it->second;
+  }
+  if (is_linear(id)) {
+    static const std::map<std::string, Role> m = {
+        {"x", Role::A}, {"w", Role::B}, {"out", Role::C}, {"bias", Role::BiasVec}, {"residual", Role::Residual},
+        {"pre", Role::Pre}, {"w_gate", Role::B}, {"w_up", Role::B2}, {"pre_gate", Role::Pre}, {"pre_up", Role::Pre2},
+        {"x2", Role::A2}, {"w2", Role::B2}, {"out2", Role::C2}, {"m", Role::M}, {"n", Role::N}, {"k", Role::K},
+        {"stride_xm", Role::StrideAm}, {"stride_xk", Role::StrideAk}, {"stride_wk", Role::StrideBk},
+        {"stride_wn", Role::StrideBn}, {"stride_om", Role::StrideCm}, {"stride_rm", Role::StrideRm},
+        {"stride_pm", Role::StridePm}};
+    auto it = m.find(n);
+    return it == m.end() ? Role::Unknown : it->second;
+  }
+  if (is_feed_forward(id)) {
+    static const std::map<std::string, Role> m = {
+        {"dout", Role::DOut}, {"pre", Role::Pre}, {"pre_gate", Role::Pre}, {"pre_up", Role::Pre2}, {"dz", Role::Dz},
+        {"dup", Role::Dz2}, {"m", Role::M}, {"n", Role::N}, {"stride_dout", Role::StrideCm},
+        {"stride_pre", Role::StridePm}, {"stride_dz", Role::StrideRm},
+        {"residual", Role::Residual}, {"block", Role::Block}, {"weight", Role::Weight}, {"bias", Role::BiasVec},
+        {"gate", Role::Gate}, {"post_weight", Role::PostWeight}, {"sum", Role::Sum}, {"normed", Role::C},
+        {"stats", Role::Stats}, {"scale", Role::Scale}, {"eps", Role::Eps}, {"d", Role::N},
+        {"stride_row", Role::StrideAm}, {"dnormed", Role::DOut}, {"dsum", Role::DSum},
+        {"dresidual", Role::DResidual}, {"dblock", Role::DBlock}, {"dweight", Role::DWeight},
+        {"dbias", Role::DBias}, {"dpost_weight", Role::DPost}};
+    if (n == "dgate") return id == KernelId::GatedActBwd ? Role::Dz : Role::DGate;
     auto it = m.find(n);
     return it == m.end() ? Role::Unknown : it->second;
   }
@@ -191,6 +233,7 @@ bool assign_positional(KernelDesc& d, std::string& err) {
       set({Role::A, Role::B, Role::BiasVec, Role::C, Role::M, Role::K, Role::N});
       return true;
     default:
+      if (is_feed_forward(d.id)) return fail("takes its arguments by name: one of them is unknown or repeated");
       return fail("is not a known entry");
   }
 }
@@ -204,7 +247,7 @@ bool check_roles(const KernelDesc& d, std::string& err) {
     for (auto& a : d.args) if (a.role == r) return true;
     return false;
   };
-  std::vector<Role> need;
+  std::vector<Role> need, may;
   switch (d.id) {
     case KernelId::Matmul: need = {Role::A, Role::B, Role::C, Role::M, Role::N, Role::K}; break;
     case KernelId::AttnFwd:
@@ -230,7 +273,52 @@ bool check_roles(const KernelDesc& d, std::string& err) {
     case KernelId::SaeEncode:
       need = {Role::A, Role::B, Role::BiasVec, Role::C, Role::M, Role::K, Role::N};
       break;
+    case KernelId::Linear:
+      need = {Role::A, Role::B, Role::C, Role::M, Role::N, Role::K};
+      may = {Role::BiasVec, Role::Residual, Role::Pre, Role::StrideAm, Role::StrideAk, Role::StrideBk, Role::StrideBn,
+             Role::StrideCm, Role::StrideRm, Role::StridePm};
+      break;
+    case KernelId::GatedLinear:
+      need = {Role::A, Role::B, Role::B2, Role::C, Role::M, Role::N, Role::K};
+      may = {Role::Pre, Role::Pre2, Role::StrideAm, Role::StrideAk, Role::StrideBk, Role::StrideBn, Role::StrideCm,
+             Role::StridePm};
+      break;
+    case KernelId::LinearSum:
+    case KernelId::LinearPair:
+      need = {Role::A, Role::B, Role::A2, Role::B2, Role::C, Role::M, Role::N, Role::K};
+      if (d.id == KernelId::LinearPair) need.push_back(Role::C2);
+      may = {Role::StrideAm, Role::StrideAk, Role::StrideBk, Role::StrideBn, Role::StrideCm};
+      break;
+    case KernelId::ActBwd:
+      need = {Role::DOut, Role::M, Role::N};
+      may = {Role::Pre, Role::Dz, Role::DBias, Role::StrideCm, Role::StridePm, Role::StrideRm};
+      break;
+    case KernelId::GatedActBwd:
+      need = {Role::DOut, Role::Pre, Role::Pre2, Role::Dz, Role::Dz2, Role::M, Role::N};
+      may = {Role::StrideCm, Role::StridePm, Role::StrideRm};
+      break;
+    case KernelId::ResidualNorm:
+      need = {Role::Residual, Role::Weight, Role::C, Role::Scale, Role::Eps, Role::M, Role::N};
+      may = {Role::Block, Role::BiasVec, Role::Gate, Role::PostWeight, Role::Sum, Role::Stats, Role::StrideAm};
+      break;
+    case KernelId::ResidualNormBwd:
+      need = {Role::DOut, Role::Sum, Role::Stats, Role::Weight, Role::Scale, Role::M, Role::N};
+      may = {Role::DSum, Role::Block, Role::Gate, Role::PostWeight, Role::DResidual, Role::DBlock, Role::DWeight,
+             Role::DBias, Role::DGate, Role::DPost, Role::StrideAm};
+      break;
     default: break;
+  }
+  if (is_feed_forward(d.id)) {
+    // optional operands: anything outside the two lists is refused
+    for (auto& a : d.args) {
+      const bool known = std::find(need.begin(), need.end(), a.role) != need.end() ||
+                         std::find(may.begin(), may.end(), a.role) != may.end();
+      if (!known) {
+        err = std::string("lowering error at line 0, col 0: ") + kernel_entry_name(d.id) + " takes no argument '" +
+              a.name + "'";
+        return false;
+      }
+    }
   }
   {
     std::set<int> once;
@@ -256,7 +344,7 @@ bool check_roles(const KernelDesc& d, std::string& err) {
       case Role::O: case Role::DO: case Role::DQ: case Role::DK: case Role::DV: case Role::L:
       case Role::Delta: case Role::In0: case Role::In1: case Role::Out: case Role::BiasVec:
         want_ptr = true; break;
-      default: break;
+      default: want_ptr = (int)a.role >= (int)Role::A2 && (int)a.role <= (int)Role::DPost; break;
     }
     if (want_ptr != a.is_pointer) {
       err = std::string("lowering error at line 0, col 0: argument ") + std::to_string(a.index) +
@@ -264,11 +352,16 @@ bool check_roles(const KernelDesc& d, std::string& err) {
             (want_ptr ? "pointer" : "scalar");
       return false;
     }
-    if ((a.role == Role::L || a.role == Role::Delta) && a.dtype != "f32") {
+    if (is_f32_role(a.role) && a.dtype != "f32") {
       err = "unsupported type '" + a.dtype + "' at line 0, col 0";
       return false;
     }
-    if ((a.role == Role::SmScale || a.role == Role::Scale || a.role == Role::Bias) && a.dtype != "f32") {
+    const bool f32_scalar = a.role == Role::SmScale || a.role == Role::Scale || a.role == Role::Bias || a.role == Role::Eps;
+    if (f32_scalar && a.dtype != "f32") {
+      err = "unsupported type '" + a.dtype + "' at line 0, col 0";
+      return false;
+    }
+    if (is_feed_forward(d.id) && !a.is_pointer && !f32_scalar && a.dtype != "i32" && a.dtype != "i64") {
       err = "unsupported type '" + a.dtype + "' at line 0, col 0";
       return false;
     }
@@ -393,7 +486,9 @@ bool scan_module(const std::string& ttir, int num_simdgroups, std::vector<Kernel
       error = "unimplemented: kernel '" + name + "' at " + loc_str(loc_of(ttir, header)) +
               " has no sm_100a implementation in libtmcuda (available: add_kernel, attn_bwd_dkdv, "
               "attn_bwd_dq, attn_bwd_preprocess, attn_fwd, copy_kernel, matmul_kernel, mul_kernel, "
-              "sae_encode_kernel, scale_bias_kernel, softmax_kernel)";
+              "sae_encode_kernel, scale_bias_kernel, softmax_kernel, activation_bwd_kernel, "
+              "gated_activation_bwd_kernel, gated_linear_kernel, linear_kernel, linear_pair_kernel, "
+              "linear_sum_kernel, residual_norm_bwd_kernel, residual_norm_kernel)";
       return false;
     }
     auto pieces = split_top(ttir.substr(open + 1, close - open - 1), open + 1);
@@ -438,7 +533,7 @@ bool scan_module(const std::string& ttir, int num_simdgroups, std::vector<Kernel
       return false;
     }
     for (auto& a : d.args) {
-      bool data_ptr = a.is_pointer && a.role != Role::L && a.role != Role::Delta;
+      bool data_ptr = a.is_pointer && !is_f32_role(a.role);
       if (data_ptr && a.dtype != e0) {
         error = "lowering error at " + loc_str(loc_of(ttir, header)) +
                 ": tt.dot operands and result must share one element type, found '" + e0 +
@@ -516,19 +611,55 @@ bool scan_module(const std::string& ttir, int num_simdgroups, std::vector<Kernel
       if (colon != std::string::npos && parse_tensor_2d(body, colon, a0, a1, te, &p1) &&
           parse_tensor_2d(body, p1, b0, b1, te, &p2)) {
         // lhs [a0 x a1] * rhs [b0 x b1]
-        if (d.id == KernelId::Matmul || d.id == KernelId::SaeEncode) { d.block_m = a0; d.block_k = a1; d.block_n = b1; }
+        if (d.id == KernelId::Matmul || d.id == KernelId::SaeEncode || is_linear(d.id)) { d.block_m = a0; d.block_k = a1; d.block_n = b1; }
         else if (d.id == KernelId::AttnBwdDkdv) { d.block_n = a0; d.head_dim = a1; d.block_m = b1; }
         else { d.block_m = a0; d.head_dim = a1; d.block_n = b1; }
       }
     } else if (parse_tensor_2d(body, 0, r0, r1, te, nullptr)) {
-      d.block_m = r0; d.head_dim = r1;
+      d.block_m = r0;
+      if (is_feed_forward(d.id)) d.block_n = r1;
+      else d.head_dim = r1;
     }
     d.threads = std::min(1024, std::max(32, num_simdgroups <= 0 ? 32 : num_simdgroups * 32));
     // an optional attribute on the function selects causal masking
     // (`tt.func @attn_fwd(...) attributes {tm.causal = true} {`): everything between the
     // argument list and the first SSA value of the body is the attribute dictionary.
     size_t first_value = body.find('%');
-    if (body.substr(0, first_value).find("tm.causal = true") != std::string::npos) d.causal = 1;
+    const std::string attributes = body.substr(0, first_value);
+    if (attributes.find("tm.causal = true") != std::string::npos) d.causal = 1;
+    if (is_feed_forward(d.id)) {
+      // tm.activation = "gelu", tm.norm = "layer" | "rms"
+      auto text_attribute = [&](const char* key) {
+        const size_t k = attributes.find(key);
+        if (k == std::string::npos) return std::string();
+        const size_t q0 = attributes.find('"', k), q1 = q0 == std::string::npos ? q0 : attributes.find('"', q0 + 1);
+        return q1 == std::string::npos ? std::string("?") : attributes.substr(q0 + 1, q1 - q0 - 1);
+      };
+      const std::string act = text_attribute("tm.activation"), norm = text_attribute("tm.norm");
+      if (!act.empty()) {
+        d.activation = has_activation(d.id) ? activation_from_name(act) : -1;
+        if (d.activation < 0) {
+          error = "unimplemented: activation '" + act + "' of '" + name + "' at " + loc_str(loc_of(ttir, header)) +
+                  " (none, relu, gelu, gelu_tanh, silu, sigmoid)";
+          return false;
+        }
+      }
+      if (!norm.empty()) {
+        if (!is_norm(d.id) || (norm != "layer" && norm != "rms")) {
+          error = "unimplemented: norm '" + norm + "' of '" + name + "' at " + loc_str(loc_of(ttir, header)) +
+                  " (rms, layer)";
+          return false;
+        }
+        d.layer_norm = norm == "layer";
+      }
+      const bool products = is_linear(d.id);
+      if (d.block_m <= 0 || d.block_n <= 0 || (products && dot == std::string::npos) ||
+          body.find("tt.store") == std::string::npos) {
+        error = "unimplemented: the body of '" + name + "' at " + loc_str(loc_of(ttir, header)) +
+                " is not the computation libtmcuda's precompiled " + kernel_entry_name(d.id) + " performs";
+        return false;
+      }
+    }
     out.push_back(d);
     pos = close;
   }
@@ -555,6 +686,8 @@ std::string descriptor_text(const std::vector<KernelDesc>& kernels) {
     o << "  block_m " << k.block_m << "\n  block_n " << k.block_n << "\n  block_k " << k.block_k
       << "\n  head_dim " << k.head_dim << "\n  threads " << k.threads << "\n  causal " << k.causal
       << "\n";
+    if (k.activation) o << "  activation " << kActivationNames[k.activation] << "\n";
+    if (k.layer_norm) o << "  norm layer\n";
     for (auto& a : k.args) {
       o << "  arg " << a.index << " " << (a.is_pointer ? "pointer" : "scalar") << " " << a.dtype
         << " " << (int)a.role << " " << (a.name.empty() ? "_" : a.name) << "\n";
@@ -609,6 +742,17 @@ bool parse_descriptor(const std::string& text, std::vector<KernelDesc>& out, std
     else if (key == "head_dim") { ls >> cur.head_dim; }
     else if (key == "threads") { ls >> cur.threads; }
     else if (key == "causal") { ls >> cur.causal; }
+    else if (key == "activation") {
+      std::string name;
+      ls >> name;
+      cur.activation = has_activation(cur.id) ? activation_from_name(name) : -1;
+      if (cur.activation < 0) return bad(t);
+    } else if (key == "norm") {
+      std::string name;
+      ls >> name;
+      if (!is_norm(cur.id) || name != "layer") return bad(t);
+      cur.layer_norm = 1;
+    }
     else if (key == "arg") {
       ArgInfo a;
       std::string kind;
@@ -634,7 +778,7 @@ bool parse_descriptor(const std::string& text, std::vector<KernelDesc>& out, std
         return false;
       }
       for (auto& a : cur.args) {
-        const bool data_ptr = a.is_pointer && a.role != Role::L && a.role != Role::Delta;
+        const bool data_ptr = a.is_pointer && !is_f32_role(a.role);
         if (data_ptr && a.dtype != elt_name(cur.elt)) {
           error = "metal error: MSL compilation failed: descriptor of " +
                   std::string(kernel_entry_name(cur.id)) + " mixes element types";

@@ -6,6 +6,7 @@
 #include "../../include/tm.h"
 #include "tm_core.h"
 #include "attn_schedule.h"
+#include "ffn_core.h"
 
 #include <algorithm>
 #include <atomic>
@@ -89,12 +90,13 @@ struct BufferObj : Object {
   bool host_exposed = false;   // tm_buffer_contents handed the pointer to the host
   bool device_only = false;    // plain device memory (tmx_alloc_device_buffer): no host pointer
   bool imported = false;       // another process's device memory, mapped by tmx_ipc_import
+  bool borrowed = false;       // an address handed to tmx_launch_on: the caller's memory
   // Ordering of tmx_buffer_write_async (which runs on a stream of its own) against the rest:
   uint64_t last_launch = 0;    // number of the last launch that took this buffer as an argument
   bool read_async_since_write = false;   // a tmx_buffer_read_async of it may still be in flight
   BufferObj() : Object(ObjKind::Buffer) {}
   ~BufferObj() override {
-    if (!ptr) return;
+    if (!ptr || borrowed) return;
     if (imported) cudaIpcCloseMemHandle(ptr);
     else cudaFree(ptr);
   }
@@ -338,8 +340,9 @@ struct Decoded {
   float sm_scale = 0.f;
 };
 
+// `lengths` (tmx_launch_on only) admits kind 4: a device address with that many bytes behind it.
 bool decode_args(KernelObj& k, const int32_t* kinds, const int64_t* values, int32_t argc,
-                 Decoded& out, std::string& err) {
+                 Decoded& out, std::string& err, const int64_t* lengths = nullptr) {
   if (argc > 0 && (!kinds || !values)) {
     err = invalid_argument("tm_launch received NULL argument arrays");
     return false;
@@ -347,7 +350,7 @@ bool decode_args(KernelObj& k, const int32_t* kinds, const int64_t* values, int3
   // Kinds are validated for every position first, as the reference does while
   // it builds its argument list (Compiler.swift:419-436).
   for (int i = 0; i < argc; ++i) {
-    if (kinds[i] < 0 || kinds[i] > 3) {
+    if (kinds[i] < 0 || kinds[i] > (lengths ? 4 : 3)) {
       err = invalid_argument("unknown launch argument kind " + std::to_string(kinds[i]) +
                              " at position " + std::to_string(i));
       return false;
@@ -362,7 +365,13 @@ bool decode_args(KernelObj& k, const int32_t* kinds, const int64_t* values, int3
   }
   for (int i = 0; i < argc; ++i) {
     const ArgInfo& a = args[i];
-    if (a.is_pointer) {
+    if (a.is_pointer && kinds[i] == 4) {
+      auto b = std::make_shared<BufferObj>();
+      b->ptr = (void*)(uintptr_t)values[i];
+      b->length = lengths[i];
+      b->borrowed = true;
+      out.buffers[(int)a.role] = b;
+    } else if (a.is_pointer) {
       if (kinds[i] != 0) {
         err = invalid_argument("argument " + std::to_string(i) + " of " +
                                kernel_entry_name(k.desc.id) + " is a pointer; expected kind 0, got " +
@@ -556,6 +565,274 @@ bool enqueue_binary(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t th
   return true;
 }
 
+// ---- the feed-forward kernels -----------------------------------------------------------------
+
+// The elements of one operand: `rows` rows `row_stride` apart of `cols` elements `col_stride` apart.
+struct Region {
+  const char* name;
+  const void* base;
+  int64_t rows, cols, row_stride, col_stride;
+};
+
+// Whether two operands share an element.  Rows of equal pitch that lie side by side (two column
+// ranges of one wider tensor) are told apart; anything else goes by the byte ranges.
+bool regions_overlap(const Region& a, const Region& b, int eb) {
+  if (!a.base || !b.base || a.rows <= 0 || a.cols <= 0 || b.rows <= 0 || b.cols <= 0) return false;
+  auto end = [&](const Region& r) {
+    return (__int128)(uintptr_t)r.base +
+           ((__int128)(r.rows - 1) * r.row_stride + (__int128)(r.cols - 1) * r.col_stride + 1) * eb;
+  };
+  const __int128 a0 = (uintptr_t)a.base, b0 = (uintptr_t)b.base;
+  if (a0 >= end(b) || b0 >= end(a)) return false;
+  if (a.col_stride == 1 && b.col_stride == 1 && a.row_stride == b.row_stride && a.row_stride > 0) {
+    const __int128 pitch = (__int128)a.row_stride * eb;
+    __int128 off = (b0 - a0) % pitch;
+    if (off < 0) off += pitch;
+    if (off >= (__int128)a.cols * eb && off + (__int128)b.cols * eb <= pitch) return false;
+  }
+  return true;
+}
+
+// Outputs may not share memory with one another or with an input, except that `out` may be exactly
+// the input `in` where the kernel reads an element before the same thread writes it.
+struct InPlace {
+  const void *out, *in;
+};
+bool check_aliasing(const std::vector<Region>& outputs, const std::vector<Region>& inputs, int eb,
+                    std::initializer_list<InPlace> allowed, std::string& err) {
+  for (size_t i = 0; i < outputs.size(); ++i) {
+    const Region& o = outputs[i];
+    if (o.base && o.rows > 1 && o.row_stride < o.cols) {
+      err = invalid_argument(std::string("rows of ") + o.name + " overlap (row stride " +
+                             std::to_string(o.row_stride) + ")");
+      return false;
+    }
+    for (size_t j = i + 1; j < outputs.size(); ++j) {
+      if (regions_overlap(o, outputs[j], eb)) {
+        err = invalid_argument(std::string(o.name) + " and " + outputs[j].name + " overlap in memory");
+        return false;
+      }
+    }
+    for (const Region& in : inputs) {
+      if (!regions_overlap(o, in, eb)) continue;
+      bool fine = false;
+      for (const InPlace& a : allowed)
+        fine = fine || (a.out == o.base && a.in == in.base && o.base == in.base && o.row_stride == in.row_stride &&
+                        o.col_stride == in.col_stride && o.cols == in.cols);
+      if (!fine) {
+        err = invalid_argument(std::string(o.name) + " overlaps its input " + in.name + " in memory");
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
+// One feed-forward launch, checked: everything that can be refused is refused by plan_feed_forward,
+// which looks at no device.
+struct FeedForwardPlan {
+  bool nothing = true;   // no element to compute
+  LinearProblem linear{};
+  ActBwdProblem act{};
+  NormProblem norm{};
+};
+
+bool plan_feed_forward(const KernelObj& k, const Decoded& d, int64_t gx, int64_t gy, FeedForwardPlan& plan,
+                       std::string& err) {
+  const KernelDesc& desc = k.desc;
+  const int eb = elt_size(desc.elt);
+  auto buf = [&](Role r) -> const BufferObj* {
+    auto it = d.buffers.find((int)r);
+    return it == d.buffers.end() ? nullptr : it->second.get();
+  };
+  auto ptr = [&](Role r) -> void* { const BufferObj* b = buf(r); return b ? b->ptr : nullptr; };
+  auto number = [&](Role r, int64_t fallback, const char* name, int64_t& to) {
+    to = get_int(d, r, fallback);
+    if (to < 0) err = invalid_argument(std::string(name) + " must not be negative, got " + std::to_string(to));
+    return to >= 0;
+  };
+  auto f32 = [&](Role r) { auto it = d.floats.find((int)r); return it == d.floats.end() ? 0.f : it->second; };
+  // Every operand as rows x cols; checked against its buffer, and recorded for the aliasing check.
+  std::vector<Region> inputs, outputs;
+  auto operand = [&](Role r, const char* name, int64_t rows, int64_t cols, int64_t rs, int64_t cs, bool output,
+                     int bytes = 0) {
+    const BufferObj* b = buf(r);
+    if (!b) return true;
+    bytes = bytes ? bytes : eb;
+    if (!check_extent(*b, {{rows, rs}, {cols, cs}}, bytes, name, err)) return false;
+    if ((uintptr_t)b->ptr % (size_t)bytes) {
+      err = invalid_argument(std::string(name) + " is not aligned to its element size");
+      return false;
+    }
+    (output ? outputs : inputs).push_back(Region{name, b->ptr, rows, cols, rs, cs});
+    return true;
+  };
+  if (is_linear(desc.id)) {
+    LinearProblem& p = plan.linear;
+    p.elt = desc.elt;
+    p.act = (Act)desc.activation;
+    p.mode = desc.id == KernelId::GatedLinear ? LinearMode::Gated
+             : desc.id == KernelId::LinearSum ? LinearMode::Sum
+             : desc.id == KernelId::LinearPair ? LinearMode::Pair : LinearMode::Single;
+    int64_t M, N, K;
+    if (!number(Role::M, 0, "M", M) || !number(Role::N, 0, "N", N) || !number(Role::K, 0, "K", K) ||
+        !number(Role::StrideAm, K, "stride_xm", p.sxm) || !number(Role::StrideAk, 1, "stride_xk", p.sxk) ||
+        !number(Role::StrideBk, N, "stride_wk", p.swk) || !number(Role::StrideBn, 1, "stride_wn", p.swn) ||
+        !number(Role::StrideCm, N, "stride_om", p.som) || !number(Role::StrideRm, N, "stride_rm", p.srm) ||
+        !number(Role::StridePm, N, "stride_pm", p.spm))
+      return false;
+    if (desc.block_m > 0) M = std::min<int64_t>(M, gx * (int64_t)desc.block_m);
+    if (desc.block_n > 0) N = std::min<int64_t>(N, gy * (int64_t)desc.block_n);
+    p.M = M; p.N = N; p.K = K;
+    if (!check_int32(M, "M", err) || !check_int32(N, "N", err) || !check_int32(K, "K", err)) return false;
+    if (M == 0 || N == 0) return true;
+    const bool gated = p.mode == LinearMode::Gated;
+    if (!operand(Role::A, "x", M, K, p.sxm, p.sxk, false) || !operand(Role::A2, "x2", M, K, p.sxm, p.sxk, false) ||
+        !operand(Role::B, gated ? "w_gate" : "w", K, N, p.swk, p.swn, false) ||
+        !operand(Role::B2, gated ? "w_up" : "w2", K, N, p.swk, p.swn, false) ||
+        !operand(Role::BiasVec, "bias", 1, N, 0, 1, false) ||
+        !operand(Role::Residual, "residual", M, N, p.srm, 1, false) ||
+        !operand(Role::C, "out", M, N, p.som, 1, true) || !operand(Role::C2, "out2", M, N, p.som, 1, true) ||
+        !operand(Role::Pre, gated ? "pre_gate" : "pre", M, N, p.spm, 1, true) ||
+        !operand(Role::Pre2, "pre_up", M, N, p.spm, 1, true))
+      return false;
+    p.x = ptr(Role::A); p.x2 = ptr(Role::A2); p.w = ptr(Role::B); p.w2 = ptr(Role::B2);
+    p.bias = ptr(Role::BiasVec); p.residual = ptr(Role::Residual);
+    p.out = ptr(Role::C); p.out2 = ptr(Role::C2); p.pre = ptr(Role::Pre); p.pre2 = ptr(Role::Pre2);
+    if (!check_aliasing(outputs, inputs, eb, {{p.out, p.residual}}, err)) return false;
+  } else if (!is_norm(desc.id)) {
+    ActBwdProblem& p = plan.act;
+    p.elt = desc.elt;
+    p.act = (Act)desc.activation;
+    p.gated = desc.id == KernelId::GatedActBwd;
+    int64_t M, N;
+    if (!number(Role::M, 0, "M", M) || !number(Role::N, 0, "N", N) ||
+        !number(Role::StrideCm, N, "stride_dout", p.s_dout) || !number(Role::StridePm, N, "stride_pre", p.s_pre) ||
+        !number(Role::StrideRm, N, "stride_dz", p.s_dz))
+      return false;
+    if (desc.block_m > 0) M = std::min<int64_t>(M, gx * (int64_t)desc.block_m);
+    if (desc.block_n > 0) N = std::min<int64_t>(N, gy * (int64_t)desc.block_n);
+    p.M = M; p.N = N;
+    if (!check_int32(M, "M", err) || !check_int32(N, "N", err)) return false;
+    if (N == 0) return true;
+    if (!p.gated && p.act != Act::None && !buf(Role::Pre)) {
+      err = invalid_argument("activation_bwd_kernel needs the pre-activations for this activation");
+      return false;
+    }
+    if (!operand(Role::DOut, "dout", M, N, p.s_dout, 1, false) ||
+        !operand(Role::Pre, p.gated ? "pre_gate" : "pre", M, N, p.s_pre, 1, false) ||
+        !operand(Role::Pre2, "pre_up", M, N, p.s_pre, 1, false) ||
+        !operand(Role::Dz, p.gated ? "dgate" : "dz", M, N, p.s_dz, 1, true) ||
+        !operand(Role::Dz2, "dup", M, N, p.s_dz, 1, true) || !operand(Role::DBias, "dbias", 1, N, N, 1, true))
+      return false;
+    p.dout = ptr(Role::DOut); p.pre = ptr(Role::Pre); p.up = ptr(Role::Pre2);
+    p.dz = ptr(Role::Dz); p.dup = ptr(Role::Dz2); p.dbias = ptr(Role::DBias);
+    if (!check_aliasing(outputs, inputs, eb, {{p.dz, p.dout}, {p.dz, p.pre}, {p.dz, p.up}, {p.dup, p.dout},
+                                              {p.dup, p.pre}, {p.dup, p.up}}, err))
+      return false;
+    if (!p.dz && !p.dbias) return true;
+    if (M == 0 && !p.dbias) return true;
+  } else {
+    NormProblem& p = plan.norm;
+    p.elt = desc.elt;
+    p.layer = desc.layer_norm != 0;
+    p.scale = f32(Role::Scale);
+    p.eps = f32(Role::Eps);
+    const bool backward = desc.id == KernelId::ResidualNormBwd;
+    if (!number(Role::M, 0, "M", p.M) || !number(Role::N, 0, "D", p.D) ||
+        !number(Role::StrideAm, p.D, "stride_row", p.stride))
+      return false;
+    if (desc.block_m > 0) p.M = std::min<int64_t>(p.M, gx * (int64_t)desc.block_m);
+    if (!check_int32(p.M, "M", err)) return false;
+    if (p.D > kNormMaxColumns) {
+      err = invalid_argument(std::string(kernel_entry_name(desc.id)) + " takes rows of at most " +
+                             std::to_string(kNormMaxColumns) + " columns, got " + std::to_string(p.D));
+      return false;
+    }
+    if (!backward && !(p.eps >= 0.f)) {
+      err = invalid_argument("eps must not be negative");
+      return false;
+    }
+    const bool branch = buf(Role::Gate) || buf(Role::PostWeight);
+    if (!buf(Role::Block) && branch) {
+      err = invalid_argument("a gate or a norm behind the block needs the block's output");
+      return false;
+    }
+    if (backward && ((buf(Role::DGate) && !buf(Role::Gate)) || (buf(Role::DPost) && !buf(Role::PostWeight)))) {
+      err = invalid_argument("a gradient was asked for of a gate or post weight that is not there");
+      return false;
+    }
+    if (p.D == 0) return true;
+    const int64_t M = p.M, D = p.D, s = p.stride;
+    if (!operand(Role::Residual, "residual", M, D, s, 1, false) || !operand(Role::Block, "block", M, D, s, 1, false) ||
+        !operand(Role::Weight, "weight", 1, D, 0, 1, false) || !operand(Role::BiasVec, "bias", 1, D, 0, 1, false) ||
+        !operand(Role::Gate, "gate", 1, D, 0, 1, false) ||
+        !operand(Role::PostWeight, "post_weight", 1, D, 0, 1, false) ||
+        !operand(Role::Sum, "sum", M, D, s, 1, !backward) || !operand(Role::C, "normed", M, D, s, 1, true) ||
+        !operand(Role::DOut, "dnormed", M, D, s, 1, false) || !operand(Role::DSum, "dsum", M, D, s, 1, false) ||
+        !operand(Role::DResidual, "dresidual", M, D, s, 1, true) ||
+        !operand(Role::DBlock, "dblock", M, D, s, 1, true) || !operand(Role::DWeight, "dweight", 1, D, D, 1, true) ||
+        !operand(Role::DBias, "dbias", 1, D, D, 1, true) || !operand(Role::DGate, "dgate", 1, D, D, 1, true) ||
+        !operand(Role::DPost, "dpost_weight", 1, D, D, 1, true))
+      return false;
+    p.residual = ptr(Role::Residual); p.block = ptr(Role::Block); p.weight = ptr(Role::Weight);
+    p.bias = ptr(Role::BiasVec); p.gate = ptr(Role::Gate); p.post_weight = ptr(Role::PostWeight);
+    p.sum = ptr(Role::Sum); p.normed = ptr(Role::C);
+    p.dnormed = ptr(Role::DOut); p.dsum = ptr(Role::DSum);
+    p.dresidual = ptr(Role::DResidual); p.dblock = ptr(Role::DBlock); p.dweight = ptr(Role::DWeight);
+    p.dbias = ptr(Role::DBias); p.dgate = ptr(Role::DGate); p.dpost = ptr(Role::DPost);
+    if (!check_aliasing(outputs, inputs, eb,
+                        {{p.sum, p.residual}, {p.sum, p.block}, {p.normed, p.residual}, {p.normed, p.block},
+                         {p.dresidual, p.dsum}, {p.dresidual, p.dnormed}, {p.dblock, p.dsum}, {p.dblock, p.dnormed},
+                         {p.dblock, p.block}}, err))
+      return false;
+    if (const BufferObj* stats = buf(Role::Stats)) {
+      // four fp32 words a row, in 16-byte accesses; compared with the others as elements of their size
+      if (!check_extent(*stats, {{M, 4}, {4, 1}}, 4, "stats", err)) return false;
+      if ((uintptr_t)stats->ptr % 16) {
+        err = invalid_argument("stats is not aligned to 16 bytes");
+        return false;
+      }
+      const int64_t row = 16 / eb;
+      const Region region{"stats", stats->ptr, M, row, row, 1};
+      for (auto& list : {outputs, inputs})
+        for (const Region& r : list)
+          if (regions_overlap(region, r, eb)) {
+            err = invalid_argument(std::string("stats overlaps ") + r.name + " in memory");
+            return false;
+          }
+      p.stats = (float*)stats->ptr;
+    }
+    const bool sums = p.dweight || p.dbias || p.dgate || p.dpost;
+    if (M == 0 && !sums) return true;
+  }
+  plan.nothing = false;
+  return true;
+}
+
+bool run_feed_forward(KernelObj& k, const FeedForwardPlan& plan, int repeats, const LaunchCtx& ctx, std::string& err) {
+  if (plan.nothing) return true;
+  const KernelId id = k.desc.id;
+  std::string why;
+  bool tc = false;
+  if (k.path_option == 2 && !tc) {
+    err = invalid_argument("the tcgen05 path was required but this launch is not eligible: " + why);
+    return false;
+  }
+  for (int r = 0; r < repeats; ++r) {
+    std::string e;
+    if (is_linear(id)) e = launch_linear_simt(plan.linear, ctx);
+    else if (!is_norm(id)) e = launch_activation_bwd(plan.act, ctx);
+    else e = id == KernelId::ResidualNorm ? launch_residual_norm(plan.norm, ctx) : launch_residual_norm_bwd(plan.norm, ctx);
+    if (!e.empty()) {
+      err = cuda_error(std::string(kernel_entry_name(id)) + ": " + e);
+      return false;
+    }
+  }
+  k.last_path = tc ? 2 : 1;
+  return true;
+}
+
 bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
              const int32_t* kinds, const int64_t* values, int32_t argc, int repeats,
              std::string& err) {
@@ -586,6 +863,8 @@ bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
                            " exceeds the pipeline maximum 1024");
     return false;
   }
+  FeedForwardPlan plan;
+  if (is_feed_forward(k.desc.id) && !plan_feed_forward(k, d, gx, gy, plan, err)) return false;
   if (!bind_device(err)) return false;
   {
     const std::string& why = unusable_reason();
@@ -616,6 +895,13 @@ bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
     }
     return true;
   };
+
+  if (is_feed_forward(desc.id)) {
+    prefetch_exposed(d);
+    if (!run_feed_forward(k, plan, repeats, ctx, err)) return false;
+    note.armed = true;
+    return true;
+  }
 
   if (is_rowwise(desc.id)) {
     // ---- one-dimensional kernels: program p covers [p*BLOCK, (p+1)*BLOCK) (rows for softmax) ----
@@ -1071,6 +1357,8 @@ int64_t tm_load_kernel(int64_t library, const char* name) {
         if (std::string(force) == "simt") obj->path_option = 1;
         else if (std::string(force) == "tcgen05") obj->path_option = 2;
       }
+      // the device probe waits for the GPU, which a stream capture forbids: run it before one
+      if (is_feed_forward(k.id)) unusable_reason();
       return g_handles.insert(obj);
     }
   }
@@ -1202,12 +1490,30 @@ int32_t tmx_kernel_set_option(int64_t kernel, const char* name, int64_t value) {
   }
   std::string n(name);
   if (n == "causal") {
-    if (k->desc.id == KernelId::Matmul || k->desc.id == KernelId::AttnBwdPreprocess || is_rowwise(k->desc.id)) {
+    if (k->desc.id == KernelId::Matmul || k->desc.id == KernelId::AttnBwdPreprocess || is_rowwise(k->desc.id) ||
+        is_feed_forward(k->desc.id)) {
       store_error(invalid_argument(std::string("option 'causal' does not apply to ") +
                                    kernel_entry_name(k->desc.id)));
       return -1;
     }
     k->desc.causal = value != 0;
+    return 0;
+  }
+  if (n == "activation") {
+    if (!has_activation(k->desc.id) || value < 0 || value >= kActCount) {
+      store_error(invalid_argument(std::string("option 'activation' takes 0...5 and does not apply to every kernel (") +
+                                   kernel_entry_name(k->desc.id) + ", " + std::to_string(value) + ")"));
+      return -1;
+    }
+    k->desc.activation = (int)value;
+    return 0;
+  }
+  if (n == "layer_norm") {
+    if (!is_norm(k->desc.id)) {
+      store_error(invalid_argument(std::string("option 'layer_norm' does not apply to ") + kernel_entry_name(k->desc.id)));
+      return -1;
+    }
+    k->desc.layer_norm = value != 0;
     return 0;
   }
   if (n == "path") {
@@ -1232,6 +1538,75 @@ int32_t tmx_kernel_last_path(int64_t kernel) {
 int32_t tmx_launch_async(int64_t kernel, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
                          const int32_t* kinds, const int64_t* values, int32_t argc) {
   return do_launch(kernel, gx, gy, gz, threads, kinds, values, argc, 1, false, nullptr);
+}
+
+// A feed-forward kernel on a stream of the caller's, on memory of the caller's (see include/tm.h).
+int32_t tmx_launch_on(int64_t kernel, void* stream, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
+                      const int32_t* kinds, const int64_t* values, const int64_t* lengths, int32_t argc) {
+  std::string err;
+  auto fail = [&](const std::string& m) { store_error(m); return -1; };
+  auto k = lookup_as<KernelObj>(kernel, ObjKind::Kernel, err);
+  if (!k) return fail(err);
+  if (k->binary || !is_feed_forward(k->desc.id))
+    return fail(invalid_argument("tmx_launch_on takes the feed-forward kernels; the others run on the library's own stream"));
+  if (!lengths) return fail(invalid_argument("tmx_launch_on received no lengths"));
+  Decoded d;
+  if (!decode_args(*k, kinds, values, argc, d, err, lengths)) return fail(err);
+  if (gx <= 0 || gy <= 0 || gz <= 0) return fail(invalid_argument("threadgroup grid must be positive in every dimension"));
+  if (threads <= 0 || threads > 1024) return fail(invalid_argument("threadsPerThreadgroup must be 1...1024"));
+  for (int i = 0; i < argc; ++i)
+    if (kinds[i] == 4 && (lengths[i] < 0 || (values[i] == 0 && lengths[i] > 0)))
+      return fail(invalid_argument("argument " + std::to_string(i) + " has no valid address and length"));
+  FeedForwardPlan plan;
+  if (!plan_feed_forward(*k, d, gx, gy, plan, err)) return fail(err);
+  if (!ensure_device(err)) return fail(err);
+  // the caller's current device is left as it was
+  struct Restore {
+    int device = -1;
+    ~Restore() { if (device >= 0) cudaSetDevice(device); }
+  } restore;
+  int current = -1;
+  if (cudaGetDevice(&current) == cudaSuccess && current != g_dev.ordinal) {
+    restore.device = current;
+    cudaSetDevice(g_dev.ordinal);
+  }
+  {
+    const std::string& why = unusable_reason();
+    if (!why.empty()) return fail(cuda_error(why));
+  }
+  for (int i = 0; i < argc; ++i) {
+    if (kinds[i] == 0 && stream != (void*)g_dev.stream)
+      return fail(invalid_argument("argument " + std::to_string(i) + " is a buffer of the library, which is ordered by "
+                                   "the library's stream; pass that stream, or device addresses (kind 4)"));
+    if (kinds[i] != 4 || values[i] == 0) continue;
+    cudaPointerAttributes attr{};
+    const cudaError_t e = cudaPointerGetAttributes(&attr, (const void*)(uintptr_t)values[i]);
+    if (e != cudaSuccess) cudaGetLastError();
+    if (e != cudaSuccess || (attr.type != cudaMemoryTypeDevice && attr.type != cudaMemoryTypeManaged) ||
+        attr.device != g_dev.ordinal)
+      return fail(invalid_argument("argument " + std::to_string(i) + " is not memory of device " +
+                                   std::to_string(g_dev.ordinal)));
+  }
+  LaunchCtx ctx = launch_ctx();
+  ctx.stream = (cudaStream_t)stream;
+  if (stream == (void*)g_dev.stream) {
+    prefetch_exposed(d);
+    for (auto& kv : d.buffers) {
+      if (kv.second->read_async_since_write) {
+        cudaEventRecord(g_dev.ev_order, g_dev.read_stream);
+        cudaStreamWaitEvent(g_dev.stream, g_dev.ev_order, 0);
+        break;
+      }
+    }
+  }
+  if (!run_feed_forward(*k, plan, 1, ctx, err)) return fail(err);
+  if (stream == (void*)g_dev.stream) {
+    std::vector<BufferObj*> raw;
+    for (auto& kv : d.buffers)
+      if (!kv.second->borrowed) raw.push_back(kv.second.get());
+    note_launch(raw);
+  }
+  return 0;
 }
 
 int32_t tmx_launch_timed(int64_t kernel, int64_t gx, int64_t gy, int64_t gz, int64_t threads,

@@ -35,8 +35,27 @@ enum class KernelId : int {
   // The fused sparse-autoencoder encoder, out = relu(x @ w + bias), fp32, row-major
   // (Sources/TritonMetalMLX/SAEEncoder.swift:40-200): the matmul with an epilogue.
   SaeEncode = 10,    // sae_encode_kernel(x, w, bias, out, M, D, F)
-  Count = 11
+  // The feed-forward half of a transformer layer (no counterpart in the reference; ffn_core.h has
+  // their formulas).
+  Linear = 11,         // out = act(x w + bias) + residual
+  GatedLinear = 12,    // out = act(x w_gate) * (x w_up)
+  LinearSum = 13,      // out = x w + x2 w2
+  LinearPair = 14,     // out = x w, out2 = x2 w2
+  ActBwd = 15,         // dz = dout act'(pre), dbias = column sums of dz
+  GatedActBwd = 16,    // dgate, dup from dout
+  ResidualNorm = 17,
+  ResidualNormBwd = 18,
+  Count = 19
 };
+inline bool is_linear(KernelId id) {
+  return (int)id >= (int)KernelId::Linear && (int)id <= (int)KernelId::LinearPair;
+}
+inline bool is_norm(KernelId id) { return id == KernelId::ResidualNorm || id == KernelId::ResidualNormBwd; }
+inline bool is_feed_forward(KernelId id) { return (int)id >= (int)KernelId::Linear && (int)id < (int)KernelId::Count; }
+// those whose formula has an activation
+inline bool has_activation(KernelId id) {
+  return id == KernelId::Linear || id == KernelId::GatedLinear || id == KernelId::ActBwd || id == KernelId::GatedActBwd;
+}
 inline bool is_rowwise(KernelId id) {
   return (int)id >= (int)KernelId::VecCopy && (int)id <= (int)KernelId::Softmax;
 }
@@ -54,8 +73,13 @@ enum class Role : int {
   In0, In1, Out, Count, Scale, Bias, StrideIn, StrideOut, NCols,
   // sae_encode_kernel (x, w, out, M, D, F reuse A, B, C, M, K, N)
   BiasVec,
-  Last = BiasVec
+  // feed-forward kernels (x, w, out and M, N, K with their strides reuse A, B, C ...)
+  A2, B2, C2, Residual, Pre, Pre2, Block, Gate, PostWeight, Weight, Sum, Stats,
+  DOut, DSum, Dz, Dz2, DResidual, DBlock, DWeight, DBias, DGate, DPost, Eps, StrideRm, StridePm,
+  Last = StridePm
 };
+// Pointers whose element type is f32 whatever the kernel's.
+inline bool is_f32_role(Role r) { return r == Role::L || r == Role::Delta || r == Role::Stats; }
 
 struct ArgInfo {
   int index = 0;
@@ -72,6 +96,8 @@ struct KernelDesc {
   int block_m = 0, block_n = 0, block_k = 0, head_dim = 0;
   int threads = 128;
   int causal = 0;
+  int activation = 0;   // tmc::Act, feed-forward kernels
+  int layer_norm = 0;   // 1: layer norm, 0: root-mean-square norm
   std::vector<ArgInfo> args;
 };
 
@@ -82,6 +108,8 @@ bool scan_module(const std::string& ttir, int num_simdgroups,
                  std::vector<KernelDesc>& out, std::string& error);
 std::string descriptor_text(const std::vector<KernelDesc>& kernels);
 bool parse_descriptor(const std::string& text, std::vector<KernelDesc>& out, std::string& error);
+// "none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid" -> 0...5, or -1.
+int activation_from_name(const std::string& name);
 std::string kernel_info_json(const std::vector<KernelDesc>& kernels);
 
 // ---------------------------------------------------------------------------

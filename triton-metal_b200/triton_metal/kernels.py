@@ -10,6 +10,7 @@ Argument order is the Python order of python/examples/attention_training.py and
 python/examples/matmul.py with all six strides present.
 """
 
+import ctypes
 import math
 
 from . import _core, cuda, launcher
@@ -211,6 +212,34 @@ def sae_encode_ir(block_m=64, block_f=64, block_d=16):
 """
 
 
+# ---- the feed-forward kernels ---------------------------------------------------------------
+# (no counterpart in the reference; include/tm.h lists their arguments.)  Signature-level like
+# the matmul: named arguments, the optional ones present or absent, and a body that carries the
+# BLOCK shape.
+
+def feed_forward_ir(name, arguments, element="bf16", block=(128, 128), activation=None, norm=None, product=False):
+    """`arguments`: the names in order; pointers and scalars are told apart by name."""
+    e = ELEMENT[element]
+    parts = []
+    for a in arguments:
+        if a in ("M", "N", "K", "D") or a.startswith("stride_"):
+            parts.append(f"%{a}: i64")
+        elif a in ("scale", "eps"):
+            parts.append(f"%{a}: f32")
+        else:
+            parts.append(f"%{a}: !tt.ptr<{'f32' if a == 'stats' else e}>")
+    entries = ([f'tm.activation = "{activation}"'] if activation else []) + ([f'tm.norm = "{norm}"'] if norm else [])
+    attributes = f" attributes {{{', '.join(entries)}}}" if entries else ""
+    tile = f"tensor<{block[0]}x{block[1]}x{e}>"
+    if product:
+        body = (f"    %acc = tt.dot %a, %b, %zero : tensor<{block[0]}x64x{e}> * tensor<64x{block[1]}x{e}> -> "
+                f"tensor<{block[0]}x{block[1]}xf32>\n")
+    else:
+        body = f"    %v = tt.load %p : {tile}\n"
+    return (f"module {{\n  tt.func public @{name}({', '.join(parts)}){attributes} {{\n{body}"
+            f"    tt.store %q, %r : {tile}\n    tt.return\n  }}\n}}\n")
+
+
 class _Handle:
     """A bare buffer handle presented the way the launcher takes pointer arguments."""
     __slots__ = ("tm_handle",)
@@ -408,6 +437,131 @@ class Softmax(Kernel):
 
     def __call__(self, *a, **kw):
         self.launch(*self.arguments(*a, **kw))
+
+
+class FeedForwardKernel(Kernel):
+    """A kernel whose arguments go by name: called with keyword arguments (buffer handles and
+    numbers), it runs on the library's stream and waits; `launch_tensors` enqueues it on a stream of
+    the caller's with device addresses."""
+
+    NAME, REQUIRED, OPTIONAL, SCALARS, PRODUCT = "", (), (), (), False
+    ACTIVATION, NORM, COLUMNS = False, False, "N"
+
+    def __init__(self, element="bf16", operands=(), activation=None, norm=None, block=(128, 128), num_warps=4):
+        unknown = [o for o in operands if o not in self.OPTIONAL]
+        if unknown:
+            raise TypeError(f"{self.NAME} takes no operand {unknown[0]!r}; it may have {', '.join(self.OPTIONAL)}")
+        if activation is not None and (not self.ACTIVATION or activation not in cuda.ACTIVATIONS):
+            raise ValueError(f"{self.NAME}: unknown activation {activation!r}")
+        if norm is not None and (not self.NORM or norm not in ("rms", "layer")):
+            raise ValueError(f"{self.NAME}: unknown norm {norm!r}")
+        self.pointers = tuple(self.REQUIRED) + tuple(o for o in self.OPTIONAL if o in operands)
+        self.names = self.pointers + self.SCALARS
+        self.block = block
+        super().__init__(feed_forward_ir(self.NAME, self.names, element, block, activation, norm, self.PRODUCT),
+                         self.NAME, num_warps)
+        self._kinds = (ctypes.c_int32 * len(self.names))(*(
+            [cuda.ARG_DEVICE_ADDRESS] * len(self.pointers) + [
+                _core.ARG_F32 if n in ("scale", "eps") else _core.ARG_I64
+                for n in self.SCALARS]))
+        self._values = ctypes.c_int64 * len(self.names)
+
+    def _grid(self, rows, columns):
+        return (max(1, cdiv(rows, self.block[0])), max(1, cdiv(columns, self.block[1])), 1)
+
+    def arguments(self, **operands):
+        """(grid, kinds, values) for tm_launch; operands by name, strides default to dense rows."""
+        for name, value in self.dense_strides(operands).items():
+            operands.setdefault(name, value)
+        missing = [n for n in self.names if n not in operands]
+        extra = [n for n in operands if n not in self.names]
+        if missing or extra:
+            raise TypeError(f"{self.NAME}: " + (f"missing {missing[0]!r}" if missing else f"no argument {extra[0]!r}"))
+        kinds, values = self.marshal(*(operands[n] for n in self.names))
+        return self._grid(operands["M"], operands[self.COLUMNS]), kinds, values
+
+    def dense_strides(self, o):
+        return {}
+
+    def __call__(self, **operands):
+        self.launch(*self.arguments(**operands))
+
+    def launch_tensors(self, stream, pointers, lengths, scalars):
+        """Enqueue on `stream`: addresses and lengths in the order of `self.pointers`, numbers (f32 as
+        bit patterns) in the order of SCALARS."""
+        n = len(self.names)
+        rows, columns = scalars[0], scalars[1]
+        grid = (max(1, -(-rows // self.block[0])), max(1, -(-columns // self.block[1])))
+        cuda.launch_on(self.handle, stream, grid, self.threads, self._kinds, self._values(*pointers, *scalars),
+                       self._values(*lengths, *([0] * (n - len(lengths)))))
+
+
+class Linear(FeedForwardKernel):
+    """out = act(x @ w + bias) + residual; pre = x @ w + bias."""
+    NAME, PRODUCT, ACTIVATION = "linear_kernel", True, True
+    REQUIRED, OPTIONAL = ("x", "w", "out"), ("bias", "residual", "pre")
+    SCALARS = ("M", "N", "K", "stride_xm", "stride_xk", "stride_wk", "stride_wn", "stride_om", "stride_rm", "stride_pm")
+
+    def dense_strides(self, o):
+        n, k = o.get("N"), o.get("K")
+        strides = dict(stride_xm=k, stride_xk=1, stride_wk=n, stride_wn=1, stride_om=n, stride_rm=n, stride_pm=n)
+        return {name: strides[name] for name in self.SCALARS if name in strides}
+
+
+class GatedLinear(Linear):
+    """out = act(x @ w_gate) * (x @ w_up)."""
+    NAME = "gated_linear_kernel"
+    REQUIRED, OPTIONAL = ("x", "w_gate", "w_up", "out"), ("pre_gate", "pre_up")
+    SCALARS = ("M", "N", "K", "stride_xm", "stride_xk", "stride_wk", "stride_wn", "stride_om", "stride_pm")
+
+
+class LinearSum(Linear):
+    """out = x @ w + x2 @ w2."""
+    NAME, ACTIVATION = "linear_sum_kernel", False
+    REQUIRED, OPTIONAL = ("x", "w", "x2", "w2", "out"), ()
+    SCALARS = ("M", "N", "K", "stride_xm", "stride_xk", "stride_wk", "stride_wn", "stride_om")
+
+
+class LinearPair(LinearSum):
+    """out = x @ w, out2 = x2 @ w2."""
+    NAME = "linear_pair_kernel"
+    REQUIRED = ("x", "w", "x2", "w2", "out", "out2")
+
+
+class ActivationBackward(FeedForwardKernel):
+    """dz = dout * act'(pre); dbias = column sums of dz."""
+    NAME, ACTIVATION = "activation_bwd_kernel", True
+    REQUIRED, OPTIONAL = ("dout",), ("pre", "dz", "dbias")
+    SCALARS = ("M", "N", "stride_dout", "stride_pre", "stride_dz")
+
+    def dense_strides(self, o):
+        return {name: o.get("N") for name in ("stride_dout", "stride_pre", "stride_dz")}
+
+
+class GatedActivationBackward(ActivationBackward):
+    """dgate = dout * pre_up * act'(pre_gate); dup = dout * act(pre_gate)."""
+    NAME = "gated_activation_bwd_kernel"
+    REQUIRED, OPTIONAL = ("dout", "pre_gate", "pre_up", "dgate", "dup"), ()
+
+
+class ResidualNorm(FeedForwardKernel):
+    """sum = scale * residual + gate * t, t = N(block) * post_weight or block; normed = N(sum) * weight + bias."""
+    NAME, NORM, COLUMNS = "residual_norm_kernel", True, "D"
+    REQUIRED = ("residual", "weight", "normed")
+    OPTIONAL = ("block", "bias", "gate", "post_weight", "sum", "stats")
+    SCALARS = ("M", "D", "scale", "eps", "stride_row")
+
+    def dense_strides(self, o):
+        return {"stride_row": o.get("D")}
+
+
+class ResidualNormBackward(ResidualNorm):
+    """The gradients of ResidualNorm from those of sum and normed."""
+    NAME = "residual_norm_bwd_kernel"
+    REQUIRED = ("dnormed", "sum", "stats", "weight")
+    OPTIONAL = ("dsum", "block", "gate", "post_weight", "dresidual", "dblock", "dweight", "dbias", "dgate",
+                "dpost_weight")
+    SCALARS = ("M", "D", "scale", "stride_row")
 
 
 def default_scale(head_dim):
