@@ -814,14 +814,11 @@ bool run_feed_forward(KernelObj& k, const FeedForwardPlan& plan, int repeats, co
   if (plan.nothing) return true;
   const KernelId id = k.desc.id;
   std::string why;
-  bool tc = false;
-  if (k.path_option == 2 && !tc) {
-    err = invalid_argument("the tcgen05 path was required but this launch is not eligible: " + why);
-    return false;
-  }
-  for (int r = 0; r < repeats; ++r) {
+  int path = 1;
+  if (k.path_option == 2 && !is_linear(id)) why = "it has no matrix product";
+  for (int r = 0; r < repeats && why.empty(); ++r) {
     std::string e;
-    if (is_linear(id)) e = launch_linear_simt(plan.linear, ctx);
+    if (is_linear(id)) e = launch_linear(plan.linear, ctx, k.path_option, &path, &why);
     else if (!is_norm(id)) e = launch_activation_bwd(plan.act, ctx);
     else e = id == KernelId::ResidualNorm ? launch_residual_norm(plan.norm, ctx) : launch_residual_norm_bwd(plan.norm, ctx);
     if (!e.empty()) {
@@ -829,7 +826,11 @@ bool run_feed_forward(KernelObj& k, const FeedForwardPlan& plan, int repeats, co
       return false;
     }
   }
-  k.last_path = tc ? 2 : 1;
+  if (!why.empty()) {
+    err = invalid_argument("the tcgen05 path was required but this launch is not eligible: " + why);
+    return false;
+  }
+  k.last_path = path;
   return true;
 }
 
