@@ -20,7 +20,8 @@ EXPORTS = {
     "tmx_kernel_last_path": (_I32, (_I64,)),
     "tmx_launch_async": (_I32, _LAUNCH),
     "tmx_launch_timed": (_I32, _LAUNCH + (_I32, _F32P)),
-    "tmx_launch_on": (_I32, (_I64, _PTR, _I64, _I64, _I64, _I64, _I32P, _I64P, _I64P, _I32)),
+    # (the arrays as plain addresses: ctypes arrays or packed bytes)
+    "tmx_launch_on": (_I32, (_I64, _PTR, _I64, _I64, _I64, _I64, _PTR, _PTR, _PTR, _I32)),
     "tmx_synchronize": (_I32, ()),
     "tmx_buffer_write_async": (_I32, (_I64, _I64, _PTR, _I64)),
     "tmx_buffer_read_async": (_I32, (_I64, _I64, _PTR, _I64)),
@@ -100,7 +101,7 @@ ACTIVATIONS = ("none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid")
 
 def launch_on(kernel, stream, grid, threads, kinds, values, lengths) -> None:
     """Enqueue a feed-forward kernel on a CUDA stream of the caller's.  `kinds`, `values` and
-    `lengths` are ctypes arrays; kind ARG_DEVICE_ADDRESS passes raw device memory."""
+    `lengths` are ctypes arrays (i32, i64, i64); kind ARG_DEVICE_ADDRESS passes raw device memory."""
     _ok(_lib.tmx_launch_on(kernel, stream, grid[0], grid[1], 1, threads, kinds, values, lengths, len(kinds)))
 
 

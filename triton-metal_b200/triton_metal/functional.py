@@ -5,286 +5,374 @@
     residual_norm     sum = scale * residual + gate * post(block), normed = norm(sum) * weight + bias
 
 and their backward passes, each one or a few launches of this library's kernels (kernels.Linear,
-GatedLinear, ..., through tmx_launch_on) on torch's current stream.  Nothing waits, nothing is
-cached between calls but the loaded kernels, and a call may be captured into a CUDA graph.  All
-tensors live on the library's device and share one element type: float32, float16 or bfloat16.
+GatedLinear, ..., through tmx_launch_on) on torch's current stream.  Nothing waits, and a call may be
+captured into a CUDA graph.  All tensors live on the library's device and share one element type:
+float32, float16 or bfloat16.
 
 x may have leading dimensions ([..., K]); weights are [K, N] with either dimension contiguous, so a
 weight stored [N, K] is passed as its transposed view.  Gradients are explicit functions: they take
-what the forward pass returned and return contiguous tensors (a weight's gradient in the layout of
-the weight).  The reference has no counterpart.
+what the forward pass returned and return new tensors (a weight's gradient in the layout of the
+weight).  The reference has no counterpart.
+
+Every call goes through a recipe: the checks of shapes, types and strides, the temporaries, and the
+launches with everything but the addresses.  Recipes depend on the operands' metadata alone and are
+kept by it, so a repeated call pays for its allocations, its addresses and its launches; the library
+checks addresses (device, alignment, overlap) on every launch.
 """
 
 import math
+import struct
 
 import torch
 
 from . import _core, cuda, kernels
 
 _ELEMENT = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
-_loaded = {}
-
-
-def _kernel(cls, dtype, operands, activation=None, norm=None):
-    key = (cls, dtype, operands, activation, norm)
-    kern = _loaded.get(key)
-    if kern is None:
-        kern = _loaded[key] = cls(_ELEMENT[dtype], operands, activation, norm)
-    return kern
+_KERNELS = {}
+_RECIPES = {}
+_MOST_RECIPES = 4096
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def release():
-    """Drop the loaded kernels (they are loaded again on the next call)."""
-    for kern in _loaded.values():
+    """Drop the loaded kernels and recipes (they are made again on the next call)."""
+    _RECIPES.clear()
+    for kern in _KERNELS.values():
         kern.release()
-    _loaded.clear()
+    _KERNELS.clear()
 
 
-def _check(name, t, dtype, device, shape=None):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} is {t.dtype}, the other operands are {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the other operands are on {device}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    return t
+def _kernel(cls, dtype, operands=(), activation=None, norm=None):
+    key = (cls, dtype, operands, activation, norm)
+    kern = _KERNELS.get(key)
+    if kern is None:
+        kern = _KERNELS[key] = cls(_ELEMENT[dtype], operands, activation, norm)
+    return kern
 
 
-def _first(name, t):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
-    if t.dtype not in _ELEMENT:
-        raise TypeError(f"{name} is {t.dtype}; float32, float16 and bfloat16 are supported")
-    if not t.is_cuda or t.device.index != cuda.get_device():
-        raise ValueError(f"{name} is on {t.device}; this process's device is cuda:{cuda.get_device()}")
-    if t.dim() < 1:
-        raise ValueError(f"{name} needs at least one dimension")
-    return t.dtype, t.device
+class _Matrix:
+    """Rows and columns with two strides, in the tensor at `slot` of a recipe."""
+    __slots__ = ("slot", "rows", "cols", "s0", "s1")
+
+    def __init__(self, slot, rows, cols, s0, s1):
+        # strides of dimensions of one element are made the dense ones
+        if cols <= 1:
+            s1 = 1
+        if rows <= 1:
+            s0 = max(cols, 1) if s1 == 1 else 1
+        self.slot, self.rows, self.cols, self.s0, self.s1 = slot, rows, cols, s0, s1
+
+    @property
+    def T(self):
+        return _Matrix(self.slot, self.cols, self.rows, self.s1, self.s0)
+
+    def span(self):
+        return 0 if not self.rows or not self.cols else (self.rows - 1) * self.s0 + (self.cols - 1) * self.s1 + 1
 
 
-def _rows(name, t):
-    """[..., C] as [R, C] with unit column stride (a copy only where no view has that form)."""
-    t = t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+class _Recipe:
+    """`tensors`: the operands by name; what is None is left out."""
+
+    def __init__(self, **tensors):
+        first_name, first = next(iter(tensors.items()))
+        for name, t in tensors.items():
+            if t is not None and not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
+        if first.dtype not in _ELEMENT:
+            raise TypeError(f"{first_name} is {first.dtype}; float32, float16 and bfloat16 are supported")
+        if not first.is_cuda or first.device.index != cuda.get_device():
+            raise ValueError(f"{first_name} is on {first.device}; this process's device is cuda:{cuda.get_device()}")
+        self.dtype, self.device = first.dtype, first.device
+        self.width = first.element_size()
+        for name, t in tensors.items():
+            if t is None:
+                continue
+            if t.dtype != self.dtype and not (name == "stats" and t.dtype == torch.float32):
+                raise TypeError(f"{name} is {t.dtype}, expected {torch.float32 if name == 'stats' else self.dtype}")
+            if t.device != self.device:
+                raise ValueError(f"{name} is on {t.device}, the other operands are on {self.device}")
+        self.tensors = tensors
+        self.slots = {name: i for i, name in enumerate(tensors)}
+        self.copies, self.allocs, self.steps, self.results = [], [], [], []
+
+    # ---- operands -------------------------------------------------------------------------
+    def shape(self, name, shape):
+        t = self.tensors[name]
+        if t is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+    def rows(self, name, dense=False, writable=False):
+        """[..., C] as a matrix with unit column stride: a view where there is one, else a copy."""
+        t = self.tensors[name]
+        if t is None:
+            return None
+        if t.dim() < 1:
+            raise ValueError(f"{name} needs at least one dimension")
+        rows, cols, slot = math.prod(t.shape[:-1]), t.shape[-1], self.slots[name]
+        view = t if t.dim() == 2 else None
+        if view is None:
+            try:
+                view = t.view(rows, cols)
+            except RuntimeError:
+                pass
+        if view is not None and (view.stride(1) == 1 or cols <= 1):
+            m = _Matrix(slot, rows, cols, *view.stride())
+            if not dense or m.s0 == max(cols, 1):
+                return m
+        if writable:
+            raise ValueError(f"{name} must have contiguous rows a fixed distance apart")
+        self.copies.append((slot, (rows, cols)))
+        return _Matrix(slot, rows, cols, max(cols, 1), 1)
+
+    def matrix(self, name, rows, cols=None):
+        t = self.tensors[name]
+        if t.dim() != 2 or t.shape[0] != rows or (cols is not None and t.shape[1] != cols):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({rows}, {'N' if cols is None else cols})")
+        return _Matrix(self.slots[name], t.shape[0], t.shape[1], *t.stride())
+
+    def vector(self, name, n):
+        t = self.tensors[name]
+        if t is None:
+            return None
+        self.shape(name, (n,))
+        if t.stride(0) != 1 and n > 1:
+            self.copies.append((self.slots[name], (n,)))
+        return _Matrix(self.slots[name], 1, n, max(n, 1), 1)
+
+    def new(self, shape, dtype=None):
+        """A new dense tensor, as a matrix of its rows."""
+        slot = len(self.tensors) + len(self.allocs)
+        self.allocs.append((tuple(shape), dtype or self.dtype))
+        rows, cols = math.prod(shape[:-1]), shape[-1]
+        return _Matrix(slot, rows, cols, max(cols, 1), 1)
+
+    # ---- launches ---------------------------------------------------------------------------
+    def launch(self, cls, operands, scalars, activation=None, norm=None):
+        """`operands`: name -> matrix; None is left out.  `scalars` in the kernel's order."""
+        present = {name: m for name, m in operands.items() if m is not None}
+        kern = _kernel(cls, self.dtype, tuple(n for n in cls.OPTIONAL if n in present), activation, norm)
+        slots = [present[n].slot for n in kern.pointers]
+        n = len(kern.names)
+        lengths = [present[n_].span() * (4 if n_ == "stats" else self.width) for n_ in kern.pointers]
+        pack = struct.Struct(f"{n}q")
+        grid = kern._grid(scalars[0], scalars[1])
+        self.steps.append((kern.handle, grid[0], grid[1], kern.threads, kern._kinds, slots, tuple(scalars), pack.pack,
+                           pack.pack(*lengths, *([0] * len(scalars))), n))
+
+    def product(self, x, w, out):
+        self.launch(kernels.Linear, dict(x=x, w=w, out=out),
+                    (x.rows, w.cols, x.cols, x.s0, x.s1, w.s0, w.s1, out.s0, out.s0, out.s0))
+
+    def run(self, tensors):
+        slots = list(tensors)
+        for slot, shape in self.copies:
+            slots[slot] = slots[slot].reshape(shape).contiguous()
+        device = self.device
+        for shape, dtype in self.allocs:
+            slots.append(torch.empty(shape, dtype=dtype, device=device))
+        stream = _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+        for handle, gx, gy, threads, kinds, used, scalars, pack, lengths, n in self.steps:
+            if _launch_on(handle, stream, gx, gy, 1, threads, kinds,
+                          pack(*[slots[i].data_ptr() for i in used], *scalars), lengths, n):
+                raise RuntimeError(_core.last_error())
+        results = [None if r is None else slots[r[0]] if r[1] is None else r[1](slots[r[0]]) for r in self.results]
+        return results[0] if len(results) == 1 else tuple(results)
 
 
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+_launch_on = cuda._lib.tmx_launch_on
 
 
-def _strides(t):
-    """Both strides of a matrix; those of dimensions of one element are made the dense ones."""
-    a, b = t.stride()
-    rows, cols = t.shape
-    if cols <= 1 and rows <= 1:
-        return max(cols, 1), 1
-    if cols <= 1:
-        b = 1
-    if rows <= 1:
-        a = max(cols, 1) if b == 1 else 1
-    return a, b
+def _keep(key, recipe):
+    if len(_RECIPES) >= _MOST_RECIPES:
+        _RECIPES.clear()
+    recipe.tensors = dict.fromkeys(recipe.tensors)       # metadata only: no operand is held
+    _RECIPES[key] = recipe
+    return recipe
 
 
-def _vector(name, t, dtype, device, n):
-    if t is None:
-        return None
-    _check(name, t, dtype, device, (n,))
-    return t if t.stride(0) == 1 or n <= 1 else t.contiguous()
-
-
-def _launch(kern, tensors, scalars, device):
-    pointers, lengths = [], []
-    for t in tensors:
-        pointers.append(t.data_ptr())
-        # (an empty view has no address, whatever its storage holds)
-        lengths.append(t.untyped_storage().nbytes() - t.storage_offset() * t.element_size() if t.numel() else 0)
-    kern.launch_tensors(torch.cuda.current_stream(device).cuda_stream, pointers, lengths, scalars)
-
-
-def _weight(name, w, dtype, device, K):
-    _check(name, w, dtype, device)
-    if w.dim() != 2 or w.shape[0] != K:
-        raise ValueError(f"{name} has shape {tuple(w.shape)}, expected ({K}, N)")
-    return w
+def _call(build, static, names, tensors):
+    """Run the recipe for these operands, made by `build` on first sight of their metadata."""
+    try:
+        key = (build, static, tuple([None if t is None else (t.dtype, t.device, t.shape, t.stride()) for t in tensors]))
+        recipe = _RECIPES.get(key)
+    except AttributeError:          # not a tensor: the recipe says which
+        key = recipe = None
+    if recipe is None:
+        recipe = _Recipe(**dict(zip(names, tensors)))
+        build(recipe, *static)
+        _keep(key, recipe)
+    return recipe.run(tensors)
 
 
 def _activation(name):
     if name not in cuda.ACTIVATIONS:
         raise ValueError(f"unknown activation {name!r}; expected one of {', '.join(cuda.ACTIVATIONS)}")
-    return name
+
+
+def _transposed(t):
+    return t.t()
+
+
+# ---- linear ------------------------------------------------------------------------------------
+
+def _plan_linear(r, activation, pre):
+    _activation(activation)
+    x = r.rows("x")
+    w = r.matrix("weight", x.cols)
+    shape = tuple(r.tensors["x"].shape[:-1]) + (w.cols,)
+    r.shape("residual", shape)
+    r.shape("out", shape)
+    bias, residual = r.vector("bias", w.cols), r.rows("residual")
+    out = r.rows("out", writable=True) if r.tensors["out"] is not None else r.new(shape)
+    z = r.new(shape) if pre else None
+    r.launch(kernels.Linear, dict(x=x, w=w, out=out, bias=bias, residual=residual, pre=z),
+             (x.rows, w.cols, x.cols, x.s0, x.s1, w.s0, w.s1, out.s0, residual.s0 if residual else out.s0,
+              z.s0 if z else out.s0), activation)
+    r.results = [(out.slot, None)] + ([(z.slot, None)] if pre else [])
 
 
 def linear(x, weight, bias=None, residual=None, activation="none", *, pre=False, out=None):
     """act(x @ weight + bias) + residual; with pre=True also x @ weight + bias, which the backward
     pass of an activation reads.  `out` may be `residual` itself."""
-    dtype, device = _first("x", x)
+    return _call(_plan_linear, (activation, bool(pre)), ("x", "weight", "bias", "residual", "out"),
+                 (x, weight, bias, residual, out))
+
+
+def _weight_gradient(r, x, dz, weight):
+    """The matrix and the result of x^T dz in the layout of the weight."""
+    if weight.s0 == 1 and weight.s1 != 1:
+        dw = r.new((weight.cols, weight.rows))
+        return dw, (dz.T, x), (dw.slot, _transposed)
+    dw = r.new((weight.rows, weight.cols))
+    return dw, (x.T, dz), (dw.slot, None)
+
+
+def _plan_linear_backward(r, activation, bias):
     _activation(activation)
-    x2 = _rows("x", x)
-    M, K = x2.shape
-    _weight("weight", weight, dtype, device, K)
-    N = weight.shape[1]
-    shape = x.shape[:-1] + (N,)
-    bias = _vector("bias", bias, dtype, device, N)
-    if residual is not None:
-        _check("residual", residual, dtype, device, tuple(shape))
-        r2 = _rows("residual", residual)
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
-    else:
-        _check("out", out, dtype, device, tuple(shape))
-        if out.numel() and not (out.dim() == 2 and (out.stride(1) == 1 or N <= 1)) and not out.is_contiguous():
-            raise ValueError("out must be contiguous, or a matrix with contiguous rows")
-    o2 = out if out.dim() == 2 else out.view(M, N)
-    z = torch.empty(shape, dtype=dtype, device=device) if pre else None
-    tensors, operands = [x2, weight, o2], ()
-    if bias is not None:
-        tensors.append(bias)
-        operands += ("bias",)
-    if residual is not None:
-        tensors.append(r2)
-        operands += ("residual",)
-    if pre:
-        tensors.append(z)
-        operands += ("pre",)
-    _launch(_kernel(kernels.Linear, dtype, operands, activation), tensors,
-            (M, N, K, *_strides(x2), *_strides(weight), _row_stride(o2),
-             _row_stride(r2) if residual is not None else N, N), device)
-    return (out, z) if pre else out
-
-
-def _product(a, b, device, out=None):
-    """a @ b of matrices with any strides."""
-    M, K = a.shape
-    N = b.shape[1]
-    out = torch.empty((M, N), dtype=a.dtype, device=device) if out is None else out
-    _launch(_kernel(kernels.Linear, a.dtype, ()), (a, b, out),
-            (M, N, K, *_strides(a), *_strides(b), _row_stride(out), N, N), device)
-    return out
-
-
-def _by_columns(w):
-    """Whether a [K, N] weight is stored [N, K]."""
-    return w.stride(0) == 1 and w.stride(1) != 1
+    r.shape("x", tuple(r.tensors["dout"].shape[:-1]) + tuple(r.tensors["x"].shape[-1:]))
+    x = r.rows("x")
+    w = r.matrix("weight", x.cols)
+    r.shape("dout", tuple(r.tensors["x"].shape[:-1]) + (w.cols,))
+    dout = r.rows("dout")
+    db = r.new((w.cols,)) if bias else None
+    dz = dout
+    if activation != "none":
+        if r.tensors["pre"] is None:
+            raise ValueError(f"the backward pass of {activation} needs the pre-activations")
+        r.shape("pre", r.tensors["dout"].shape)
+        pre = r.rows("pre")
+        dz = r.new((dout.rows, w.cols))
+        r.launch(kernels.ActivationBackward, dict(dout=dout, pre=pre, dz=dz, dbias=db),
+                 (dout.rows, w.cols, dout.s0, pre.s0, dz.s0), activation)
+    elif bias:
+        r.launch(kernels.ActivationBackward, dict(dout=dout, dbias=db), (dout.rows, w.cols, dout.s0, dout.s0, dout.s0),
+                 activation)
+    dx = r.new(r.tensors["x"].shape)
+    r.product(dz, w.T, dx)
+    dw, (a, b), result = _weight_gradient(r, x, dz, w)
+    r.product(a, b, dw)
+    r.results = [(dx.slot, None), result, (db.slot, None) if bias else None]
 
 
 def linear_backward(dout, x, weight, pre=None, activation="none", *, bias=False):
     """(dx, dweight, dbias or None) of linear; the gradient of the residual is dout itself.  `pre` is
     what linear returned with pre=True (not needed without an activation)."""
-    dtype, device = _first("dout", dout)
+    return _call(_plan_linear_backward, (activation, bool(bias)), ("dout", "x", "weight", "pre"),
+                 (dout, x, weight, None if activation == "none" else pre))
+
+
+# ---- gated linear ---------------------------------------------------------------------------------
+
+def _gated_weights(r, K):
+    """Both weights with the strides of w_gate."""
+    wg = r.matrix("w_gate", K)
+    wu = r.matrix("w_up", K, wg.cols)
+    if (wg.s0, wg.s1) == (wu.s0, wu.s1):
+        return wg, wu
+    # one of the two is copied into the layout of the other: the one that is not dense rows
+    if (wg.s0, wg.s1) != (max(wg.cols, 1), 1):
+        r.copies.append((wg.slot, (wg.rows, wg.cols)))
+    if (wu.s0, wu.s1) != (max(wu.cols, 1), 1):
+        r.copies.append((wu.slot, (wu.rows, wu.cols)))
+    return (_Matrix(m.slot, m.rows, m.cols, max(m.cols, 1), 1) for m in (wg, wu))
+
+
+def _plan_gated_linear(r, activation, save):
     _activation(activation)
-    x2 = _rows("x", _check("x", x, dtype, device))
-    M, K = x2.shape
-    _weight("weight", weight, dtype, device, K)
-    N = weight.shape[1]
-    _check("dout", dout, dtype, device, tuple(x.shape[:-1]) + (N,))
-    d2 = _rows("dout", dout)
-    if activation != "none":
-        if pre is None:
-            raise ValueError(f"the backward pass of {activation} needs the pre-activations")
-        p2 = _rows("pre", _check("pre", pre, dtype, device, tuple(dout.shape)))
-    db = torch.empty(N, dtype=dtype, device=device) if bias else None
-    dz = d2
-    if activation != "none" or bias:
-        tensors, operands = [d2], ()
-        if activation != "none":
-            dz = torch.empty((M, N), dtype=dtype, device=device)
-            tensors += [p2, dz]
-            operands += ("pre", "dz")
-        if bias:
-            tensors.append(db)
-            operands += ("dbias",)
-        _launch(_kernel(kernels.ActivationBackward, dtype, operands, activation), tensors,
-                (M, N, _row_stride(d2), _row_stride(p2) if activation != "none" else N, N), device)
-    dx = _product(dz, weight.t(), device).view(x.shape)
-    if _by_columns(weight):
-        dw = _product(dz.t(), x2, device).t()
-    else:
-        dw = _product(x2.t(), dz, device)
-    return dx, dw, db
+    x = r.rows("x")
+    wg, wu = _gated_weights(r, x.cols)
+    shape = tuple(r.tensors["x"].shape[:-1]) + (wg.cols,)
+    h = r.new(shape)
+    g, u = (r.new(shape), r.new(shape)) if save else (None, None)
+    r.launch(kernels.GatedLinear, dict(x=x, w_gate=wg, w_up=wu, out=h, pre_gate=g, pre_up=u),
+             (x.rows, wg.cols, x.cols, x.s0, x.s1, wg.s0, wg.s1, h.s0, h.s0), activation)
+    r.results = [(m.slot, None) for m in ((h, g, u) if save else (h,))]
 
 
 def gated_linear(x, w_gate, w_up, activation="silu", *, save=False):
     """act(x @ w_gate) * (x @ w_up); with save=True also the two products, for the backward pass."""
-    dtype, device = _first("x", x)
+    return _call(_plan_gated_linear, (activation, bool(save)), ("x", "w_gate", "w_up"), (x, w_gate, w_up))
+
+
+def _plan_gated_linear_backward(r, activation):
     _activation(activation)
-    x2 = _rows("x", x)
-    M, K = x2.shape
-    _weight("w_gate", w_gate, dtype, device, K)
-    N = w_gate.shape[1]
-    _check("w_up", w_up, dtype, device, (K, N))
-    if _strides(w_up) != _strides(w_gate):
-        w_up = _like(w_up, w_gate)
-    shape = x.shape[:-1] + (N,)
-    h = torch.empty(shape, dtype=dtype, device=device)
-    if save:
-        g, u = torch.empty_like(h), torch.empty_like(h)
-    _launch(_kernel(kernels.GatedLinear, dtype, ("pre_gate", "pre_up") if save else (), activation),
-            (x2, w_gate, w_up, h, g, u) if save else (x2, w_gate, w_up, h),
-            (M, N, K, *_strides(x2), *_strides(w_gate), N, N), device)
-    return (h, g, u) if save else h
-
-
-def _like(t, other):
-    """A copy of t with the strides of other."""
-    copy = torch.empty_strided(other.shape, other.stride(), dtype=t.dtype, device=t.device)
-    copy.copy_(t)
-    return copy
+    r.shape("x", tuple(r.tensors["dh"].shape[:-1]) + tuple(r.tensors["x"].shape[-1:]))
+    x = r.rows("x")
+    original = r.matrix("w_gate", x.cols)
+    wg, wu = _gated_weights(r, x.cols)
+    r.shape("dh", tuple(r.tensors["x"].shape[:-1]) + (wg.cols,))
+    for name in ("pre_gate", "pre_up"):
+        r.shape(name, r.tensors["dh"].shape)
+    dh, g, u = r.rows("dh"), r.rows("pre_gate"), r.rows("pre_up")
+    if g.s0 != u.s0:
+        g, u = r.rows("pre_gate", dense=True), r.rows("pre_up", dense=True)
+    M, N, K = x.rows, wg.cols, x.cols
+    dg, du = r.new((M, N)), r.new((M, N))
+    r.launch(kernels.GatedActivationBackward, dict(dout=dh, pre_gate=g, pre_up=u, dgate=dg, dup=du),
+             (M, N, dh.s0, g.s0, dg.s0), activation)
+    dx = r.new(r.tensors["x"].shape)
+    a, b = wg.T, wu.T
+    r.launch(kernels.LinearSum, dict(x=dg, w=a, x2=du, w2=b, out=dx),
+             (M, K, N, dg.s0, dg.s1, a.s0, a.s1, dx.s0))
+    dwg, (a, b), first = _weight_gradient(r, x, dg, original)
+    dwu, (a2, b2), second = _weight_gradient(r, x, du, original)
+    r.launch(kernels.LinearPair, dict(x=a, w=b, x2=a2, w2=b2, out=dwg, out2=dwu),
+             (a.rows, b.cols, a.cols, a.s0, a.s1, b.s0, b.s1, dwg.s0))
+    r.results = [(dx.slot, None), first, second]
 
 
 def gated_linear_backward(dh, x, w_gate, w_up, pre_gate, pre_up, activation="silu"):
     """(dx, dw_gate, dw_up) of gated_linear, from the products it saved."""
-    dtype, device = _first("dh", dh)
-    _activation(activation)
-    x2 = _rows("x", _check("x", x, dtype, device))
-    M, K = x2.shape
-    _weight("w_gate", w_gate, dtype, device, K)
-    N = w_gate.shape[1]
-    _check("w_up", w_up, dtype, device, (K, N))
-    if _strides(w_up) != _strides(w_gate):
-        w_up = _like(w_up, w_gate)
-    _check("dh", dh, dtype, device, tuple(x.shape[:-1]) + (N,))
-    d2 = _rows("dh", dh)
-    g2 = _rows("pre_gate", _check("pre_gate", pre_gate, dtype, device, tuple(dh.shape)))
-    u2 = _rows("pre_up", _check("pre_up", pre_up, dtype, device, tuple(dh.shape)))
-    if _row_stride(g2) != _row_stride(u2):
-        g2, u2 = g2.contiguous(), u2.contiguous()
-    both = torch.empty((2, M, N), dtype=dtype, device=device)
-    dg, du = both[0], both[1]
-    _launch(_kernel(kernels.GatedActivationBackward, dtype, (), activation), (d2, g2, u2, dg, du),
-            (M, N, _row_stride(d2), _row_stride(g2), N), device)
-    wg, wu = w_gate.t(), w_up.t()
-    dx = torch.empty((M, K), dtype=dtype, device=device)
-    _launch(_kernel(kernels.LinearSum, dtype, ()), (dg, wg, du, wu, dx),
-            (M, K, N, *_strides(dg), *_strides(wg), max(K, 1)), device)
-    if _by_columns(w_gate):
-        dwg, dwu = (torch.empty((N, K), dtype=dtype, device=device) for _ in range(2))
-        a, b = dg.t(), du.t()
-        _launch(_kernel(kernels.LinearPair, dtype, ()), (a, x2, b, x2, dwg, dwu),
-                (N, K, M, *_strides(a), *_strides(x2), max(K, 1)), device)
-        dwg, dwu = dwg.t(), dwu.t()
-    else:
-        dwg, dwu = (torch.empty((K, N), dtype=dtype, device=device) for _ in range(2))
-        a = x2.t()
-        _launch(_kernel(kernels.LinearPair, dtype, ()), (a, dg, a, du, dwg, dwu),
-                (K, N, M, *_strides(a), *_strides(dg), max(N, 1)), device)
-    return dx.view(x.shape), dwg, dwu
+    return _call(_plan_gated_linear_backward, (activation,), ("dh", "x", "w_gate", "w_up", "pre_gate", "pre_up"),
+                 (dh, x, w_gate, w_up, pre_gate, pre_up))
 
 
-def _same_rows(tensors):
-    """Matrices with one row stride: contiguous copies of those that differ from dense rows, unless all agree."""
-    present = [t for t in tensors if t is not None]
-    first = _row_stride(present[0])
-    if all(_row_stride(t) == first for t in present):
-        return tensors, first
-    return [t if t is None else t.contiguous() for t in tensors], max(present[0].shape[1], 1)
+# ---- residual norm ----------------------------------------------------------------------------------
 
-
-def _norm_kind(kind):
+def _norm_operands(r, D, kind):
     if kind not in ("rms", "layer"):
         raise ValueError(f"unknown norm {kind!r}; expected 'rms' or 'layer'")
-    return kind
+    if r.tensors["weight"] is None:
+        raise ValueError("the norm needs its weight")
+    if r.tensors["block"] is None and (r.tensors["gate"] is not None or r.tensors["post_weight"] is not None):
+        raise ValueError("a gate or a norm behind the block needs the block's output")
+    return {name: r.vector(name, D) for name in ("weight", "gate", "post_weight")}
+
+
+def _plan_residual_norm(r, kind, scale, eps, stats):
+    residual = r.rows("residual", dense=True)
+    shape, D = r.tensors["residual"].shape, residual.cols
+    operands = _norm_operands(r, D, kind)
+    r.shape("block", shape)
+    passed = r.tensors["block"] is None and scale == 1.0     # sum is residual itself
+    total = None if passed else r.new(shape)
+    normed = r.new(shape)
+    rows = r.new((residual.rows, 4), torch.float32) if stats else None
+    operands.update(residual=residual, block=r.rows("block", dense=True), bias=r.vector("bias", D), sum=total,
+                    normed=normed, stats=rows)
+    r.launch(kernels.ResidualNorm, operands,
+             (residual.rows, D, _core.float_bits(scale), _core.float_bits(eps), max(D, 1)), None, kind)
+    r.results = [None if passed else (total.slot, None), (normed.slot, None)] + ([(rows.slot, None)] if stats else [])
 
 
 def residual_norm(residual, block=None, weight=None, bias=None, gate=None, post_weight=None, *, kind="rms", scale=1.0,
@@ -296,73 +384,36 @@ def residual_norm(residual, block=None, weight=None, bias=None, gate=None, post_
 
     Without a block (and with scale 1) sum is residual itself.  stats, [rows, 4] float32, is what the
     backward pass reads: mean and 1/deviation of each row of sum, then of block."""
-    dtype, device = _first("residual", residual)
-    _norm_kind(kind)
-    D = residual.shape[-1]
-    if weight is None:
-        raise ValueError("residual_norm needs the norm's weight")
-    weight = _vector("weight", weight, dtype, device, D)
-    bias = _vector("bias", bias, dtype, device, D)
-    gate = _vector("gate", gate, dtype, device, D)
-    post_weight = _vector("post_weight", post_weight, dtype, device, D)
-    if block is None and (gate is not None or post_weight is not None):
-        raise ValueError("a gate or a norm behind the block needs the block's output")
-    r2 = _rows("residual", residual)
-    M = r2.shape[0]
-    shape = residual.shape
-    y2 = None if block is None else _rows("block", _check("block", block, dtype, device, tuple(shape)))
-    # the results are dense, and one row stride holds for all
-    r2 = r2 if _row_stride(r2) == max(D, 1) else r2.contiguous()
-    y2 = y2 if y2 is None or _row_stride(y2) == max(D, 1) else y2.contiguous()
-    normed = torch.empty(shape, dtype=dtype, device=device)
-    total = residual if block is None and scale == 1.0 else torch.empty(shape, dtype=dtype, device=device)
-    tensors, operands = [r2, weight, normed], ()
-    rows = torch.empty((M, 4), dtype=torch.float32, device=device) if stats else None
-    for name, t in (("block", y2), ("bias", bias), ("gate", gate), ("post_weight", post_weight),
-                    ("sum", None if total is residual else total), ("stats", rows)):
-        if t is not None:
-            tensors.append(t)
-            operands += (name,)
-    _launch(_kernel(kernels.ResidualNorm, dtype, operands, None, kind), tensors,
-            (M, D, _core.float_bits(scale), _core.float_bits(eps), max(D, 1)), device)
-    return (total, normed, rows) if stats else (total, normed)
+    out = _call(_plan_residual_norm, (kind, float(scale), float(eps), bool(stats)),
+                ("residual", "block", "weight", "bias", "gate", "post_weight"),
+                (residual, block, weight, bias, gate, post_weight))
+    return out if out[0] is not None else (residual,) + out[1:]
+
+
+def _plan_residual_norm_backward(r, kind, scale, bias):
+    dn = r.rows("dnormed", dense=True)
+    shape, D = r.tensors["dnormed"].shape, dn.cols
+    operands = _norm_operands(r, D, kind)
+    for name in ("dsum", "sum", "block"):
+        r.shape(name, shape)
+    r.shape("stats", (dn.rows, 4))
+    block = r.rows("block", dense=True)
+    stats = r.rows("stats", dense=True)
+    dresidual, dweight = r.new(shape), r.new((D,))
+    dblock = r.new(shape) if block is not None else None
+    dbias = r.new((D,)) if bias else None
+    dgate = r.new((D,)) if operands["gate"] is not None else None
+    dpost = r.new((D,)) if operands["post_weight"] is not None else None
+    operands.update(dnormed=dn, dsum=r.rows("dsum", dense=True), sum=r.rows("sum", dense=True), stats=stats, block=block,
+                    dresidual=dresidual, dblock=dblock, dweight=dweight, dbias=dbias, dgate=dgate, dpost_weight=dpost)
+    r.launch(kernels.ResidualNormBackward, operands, (dn.rows, D, _core.float_bits(scale), max(D, 1)), None, kind)
+    r.results = [None if m is None else (m.slot, None) for m in (dresidual, dblock, dweight, dbias, dgate, dpost)]
 
 
 def residual_norm_backward(dnormed, dsum, total, stats, weight, block=None, gate=None, post_weight=None, *, kind="rms",
                            scale=1.0, bias=False):
     """(dresidual, dblock, dweight, dbias, dgate, dpost_weight) of residual_norm, None where the operand
     was not there.  dsum, the gradient that reaches sum past the norm, may be None."""
-    dtype, device = _first("dnormed", dnormed)
-    _norm_kind(kind)
-    D = dnormed.shape[-1]
-    shape = tuple(dnormed.shape)
-    weight = _vector("weight", weight, dtype, device, D)
-    gate = _vector("gate", gate, dtype, device, D)
-    post_weight = _vector("post_weight", post_weight, dtype, device, D)
-    if block is None and (gate is not None or post_weight is not None):
-        raise ValueError("a gate or a norm behind the block needs the block's output")
-    dn = _rows("dnormed", dnormed)
-    M = dn.shape[0]
-    _check("stats", stats, torch.float32, device, (M, 4))
-    s2 = _rows("sum", _check("sum", total, dtype, device, shape))
-    ds = None if dsum is None else _rows("dsum", _check("dsum", dsum, dtype, device, shape))
-    y2 = None if block is None else _rows("block", _check("block", block, dtype, device, shape))
-    dense = max(D, 1)
-    dn, s2, ds, y2 = (t if t is None or _row_stride(t) == dense else t.contiguous() for t in (dn, s2, ds, y2))
-    stats = stats.contiguous()
-    empty = lambda *size: torch.empty(size, dtype=dtype, device=device)  # noqa: E731
-    dresidual, dweight = empty(*shape), empty(D)
-    dblock = empty(*shape) if block is not None else None
-    dbias = empty(D) if bias else None
-    dgate = empty(D) if gate is not None else None
-    dpost = empty(D) if post_weight is not None else None
-    tensors, operands = [dn, s2, stats, weight], ()
-    for name, t in (("dsum", ds), ("block", y2), ("gate", gate), ("post_weight", post_weight),
-                    ("dresidual", dresidual), ("dblock", dblock), ("dweight", dweight), ("dbias", dbias),
-                    ("dgate", dgate), ("dpost_weight", dpost)):
-        if t is not None:
-            tensors.append(t)
-            operands += (name,)
-    _launch(_kernel(kernels.ResidualNormBackward, dtype, operands, None, kind), tensors,
-            (M, D, _core.float_bits(scale), dense), device)
-    return dresidual, dblock, dweight, dbias, dgate, dpost
+    return _call(_plan_residual_norm_backward, (kind, float(scale), bool(bias)),
+                 ("dnormed", "dsum", "sum", "stats", "weight", "block", "gate", "post_weight"),
+                 (dnormed, dsum, total, stats, weight, block, gate, post_weight))
