@@ -79,6 +79,14 @@ struct Aligned {
   }
 };
 
+// The kernel for few rows or the one for many, whichever its estimate says is done first.
+std::string launch_tensor(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw, const LaunchCtx& ctx) {
+  NarrowPlan narrow{};
+  if (plan_linear_narrow(p, lx, ctx.sm_count, &narrow) && narrow.clocks < estimate_linear_tc(p, ctx.sm_count))
+    return launch_linear_narrow(p, lx, lw, narrow, ctx);
+  return launch_linear_tc(p, lx, lw, ctx);
+}
+
 }  // namespace
 
 std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path_option, int* path_used,
@@ -101,7 +109,7 @@ std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path
     return launch_linear_simt(p, ctx);
   }
   *path_used = 2;
-  if (x_fits && w_fits) return launch_linear_tc(p, lx, lw, ctx);
+  if (x_fits && w_fits) return launch_tensor(p, lx, lw, ctx);
 
   Aligned cx, cw;
   if (!x_fits) cx.plan(p.x, p.x2, p.M, p.K, p.sxm, p.sxk);
@@ -137,7 +145,7 @@ std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path
   align_operands_kernel<<<dim3((unsigned)std::max<int64_t>(blocks, 1), (unsigned)n), 256, 0, ctx.stream>>>(jobs);
   ++*ctx.launches;
   cudaError_t err = cudaGetLastError();
-  e = err != cudaSuccess ? std::string("copy launch failed: ") + cudaGetErrorString(err) : launch_linear_tc(q, lx, lw, ctx);
+  e = err != cudaSuccess ? std::string("copy launch failed: ") + cudaGetErrorString(err) : launch_tensor(q, lx, lw, ctx);
   scratch_free(ctx, scratch);
   return e;
 }

@@ -1,0 +1,352 @@
+// The feed-forward matrix products for few rows - a decoding step, a short prompt - on the tensor cores.
+//
+//   single  z = x w + bias; out = act(z) + residual       gated  out = act(x w) * (x w2)
+//   sum     out = x w + x2 w2
+//
+// With M rows of x, M small, the weights are read once and are the bound: 2 bytes for 2 M operations.
+// So w takes the MMA's 128-row side and the rows of x, padded to 16, 32, 64 or 128, the other
+// (tcgen05.mma 128 x TOK x 16, D = (x w)^T in TMEM): a CTA owns 128 output columns, streams its part of
+// w through a shared-memory ring by TMA and pads nothing that crosses the memory bus (rows of x past M
+// are filled with zeros by the TMA).  128 columns a CTA leave most SMs idle, so a cluster of up to 8
+// CTAs splits K: each accumulates its share, leaves it in its shared memory, and finishes 1/8 (1/S) of
+// the columns from all the shares through distributed shared memory, in rank order - no workspace, no
+// atomics, the same bits every time.
+//
+//   warp 4 TMA producer, warp 5 MMA issuer, warps 0-3 read TMEM (thread = output column); all six
+//   finish the cluster's sums.  About 100 KB of ring a CTA (two CTAs an SM) keep the memory bus busy:
+//   148 x 100 KB in flight against 6.5 TB/s x 1 us.
+
+#include "ffn_math.cuh"
+#include "linear_tc.h"
+#include "sm100_ptx.cuh"
+
+#include <algorithm>
+
+namespace tmc {
+namespace {
+
+using namespace ptx;
+using namespace ffn;
+
+constexpr int BN = 128;                // output columns of a CTA
+constexpr int BK = 64;
+constexpr int NUM_THREADS = 192;
+constexpr int W_BYTES = BN * BK * 2;
+
+template <int TOK, bool GATED> struct Config {
+  static constexpr int X_BYTES = TOK * BK * 2;
+  static constexpr int STAGE_BYTES = W_BYTES * (GATED ? 2 : 1) + X_BYTES;
+  // two CTAs an SM up to 64 rows, one beyond (the shares of a cluster must fit where the ring was)
+  static constexpr int RING = TOK <= 64 ? 104 * 1024 : 196 * 1024;
+  static constexpr int STAGES = RING / STAGE_BYTES;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 2048;
+  static constexpr int TMEM_COLS = TOK * (GATED ? 2 : 1) < 32 ? 32 : TOK * (GATED ? 2 : 1);
+  static_assert(STAGES >= 2 && STAGES <= 12, "ring");
+  static_assert(TOK * BN * 4 * (GATED ? 2 : 1) <= STAGES * STAGE_BYTES, "the shares fit into the ring");
+};
+
+enum Site : uint32_t { kProdEmpty = 51, kMmaFull = 52, kEpiAccFull = 53, kDrain = 54 };
+
+struct Barriers {
+  alignas(8) uint64_t full[12];
+  alignas(8) uint64_t empty[12];
+  alignas(8) uint64_t acc_full;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct alignas(64) Maps {
+  CUtensorMap x, x2, w, w2;
+};
+
+struct Args {
+  int M, N, K;
+  int act, sum, w_mn, split;
+  const void *bias, *residual;
+  void *out, *pre, *pre2;
+  int64_t srm, som, spm;
+};
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float load_share(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+
+template <typename T, bool GATED>
+__device__ __forceinline__ void finish(const Args& a, int m, int n, float z, float up) {
+  if constexpr (GATED) {
+    if (a.pre) ((T*)a.pre)[(int64_t)m * a.spm + n] = from_f32<T>(z);
+    if (a.pre2) ((T*)a.pre2)[(int64_t)m * a.spm + n] = from_f32<T>(up);
+    z = act_forward<false>((Act)a.act, z) * up;
+  } else {
+    if (a.bias) z += to_f32(((const T*)a.bias)[n]);
+    if (a.pre) ((T*)a.pre)[(int64_t)m * a.spm + n] = from_f32<T>(z);
+    z = act_forward<false>((Act)a.act, z);
+    if (a.residual) z += to_f32(((const T*)a.residual)[(int64_t)m * a.srm + n]);
+  }
+  ((T*)a.out)[(int64_t)m * a.som + n] = from_f32<T>(z);
+}
+
+template <typename T, int TOK, bool GATED>
+__global__ void __launch_bounds__(NUM_THREADS, TOK <= 64 ? 2 : 1)
+linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a, DeviceStatus* status) {
+  using C = Config<TOK, GATED>;
+  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES;
+  constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  Barriers& bars = *reinterpret_cast<Barriers*>(smem + STAGES * STAGE_BYTES);
+  const uint32_t smem_base = smem_u32(smem);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = a.split > 1 ? cta_rank() : 0;
+  WaitCtx wc{&bars.abort_flag, status};
+
+  const int n0 = (int)(blockIdx.x / a.split) * BN, m0 = (int)blockIdx.y * TOK;
+  const int rows = min(TOK, a.M - m0);
+  const int blocks_one = (a.K + BK - 1) / BK;
+  const int blocks = a.sum ? 2 * blocks_one : blocks_one;
+  const int kb0 = (int)((int64_t)blocks * rank / a.split), kb1 = (int)((int64_t)blocks * (rank + 1) / a.split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&bars.full[s]), 1);
+      mbar_init(smem_u32(&bars.empty[s]), 1);
+    }
+    mbar_init(smem_u32(&bars.acc_full), 1);
+    bars.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(smem_u32(&bars.tmem_base), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == 4 && lane == 0) {
+    tma_prefetch_desc(&maps.x);
+    tma_prefetch_desc(&maps.w);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars.tmem_base;
+
+  bool ok = true;
+  if (warp == 4) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1, wc, kProdEmpty)) { ok = false; break; }
+        const bool other = kb >= blocks_one;                         // sum: the second pair of operands
+        const int k = (other ? kb - blocks_one : kb) * BK;
+        const uint32_t bar = smem_u32(&bars.full[stage]);
+        uint32_t dst = smem_base + stage * STAGE_BYTES;
+        mbar_expect_tx(bar, STAGE_BYTES);
+#pragma unroll
+        for (int g = 0; g < (GATED ? 2 : 1); ++g) {
+          const CUtensorMap* mw = g || other ? &maps.w2 : &maps.w;
+          if (a.w_mn) {
+            tma_load_2d(dst, mw, bar, n0, k);
+            tma_load_2d(dst + 8192, mw, bar, n0 + 64, k);
+          } else {
+            tma_load_2d(dst, mw, bar, k, n0);
+          }
+          dst += W_BYTES;
+        }
+        tma_load_2d(dst, other ? &maps.x2 : &maps.x, bar, k, m0);
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      // every copy started must have landed before the CTA leaves or the ring is reused
+      const uint32_t pending = issued < (uint32_t)STAGES ? issued : (uint32_t)STAGES;
+      for (uint32_t i = 0; i < pending; ++i) {
+        if (--stage < 0) { stage = STAGES - 1; phase ^= 1; }
+        const long long t0 = clock64();
+        while (!mbar_try_wait(smem_u32(&bars.full[stage]), phase)) {
+          if (clock64() - t0 > kWaitCycles) { report_timeout(wc, kDrain, stage); break; }
+        }
+      }
+    }
+  } else if (warp == 5) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr uint32_t n_field = TOK;
+    const uint32_t idesc = make_idesc(FMT, BN, n_field, a.w_mn, 0);
+    const SmemDesc w_base = make_desc_sw128(smem_base, a.w_mn ? 8192 : 0, 1024);
+    const SmemDesc x_base = make_desc_sw128(smem_base + W_BYTES * (GATED ? 2 : 1), 0, 1024);
+    const uint32_t w_step = a.w_mn ? 2048 : 32;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(smem_u32(&bars.full[stage]), phase, wc, kMmaFull)) { ok = false; break; }
+      tc_fence_after();
+      const SmemDesc w_desc = w_base.advanced(stage * STAGE_BYTES);
+      const SmemDesc x_desc = x_base.advanced(stage * STAGE_BYTES);
+#pragma unroll
+      for (int k = 0; k < BK / 16; ++k) {
+        mma_f16_ss_elect(tmem_base, w_desc.at(k * w_step), x_desc.at(k * 32), idesc, kb > kb0 || k != 0);
+        if constexpr (GATED)
+          mma_f16_ss_elect(tmem_base + TOK, w_desc.at(W_BYTES + k * w_step), x_desc.at(k * 32), idesc, kb > kb0 || k != 0);
+      }
+      mma_commit_elect(smem_u32(&bars.empty[stage]));
+      if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    }
+    if (ok) mma_commit_elect(smem_u32(&bars.acc_full));
+  } else {
+    // ------------------------------------------------------------ accumulator, thread = output column
+    ok = mbar_wait(smem_u32(&bars.acc_full), 0, wc, kEpiAccFull);
+    tc_fence_after();
+    const uint32_t lanes = tmem_base + ((uint32_t)(warp * 32) << 16);
+    const int n = n0 + warp * 32 + lane;
+    float* share = reinterpret_cast<float*>(smem);       // [GATED][row][128 columns]: the ring is idle now
+#pragma unroll 1
+    for (int t = 0; t < rows && __all_sync(0xffffffffu, ok); t += 16) {
+      uint32_t z[16], up[16];
+      tmem_ld_32x16(lanes + t, z);
+      if constexpr (GATED) tmem_ld_32x16(lanes + TOK + t, up);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (t + i >= rows) break;
+        const float v = __uint_as_float(z[i]), u = GATED ? __uint_as_float(up[i]) : 0.f;
+        if (a.split > 1) {
+          share[(t + i) * BN + warp * 32 + lane] = v;
+          if constexpr (GATED) share[(TOK + t + i) * BN + warp * 32 + lane] = u;
+        } else if (n < a.N) {
+          finish<T, GATED>(a, m0 + t + i, n, v, u);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+  if (a.split > 1) {
+    cluster_sync();                    // every share is written
+    const int width = BN / a.split;
+    for (int i = threadIdx.x; i < rows * width; i += NUM_THREADS) {
+      const int t = i / width, c = (int)rank * width + i % width;
+      if (n0 + c >= a.N) continue;
+      const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
+      float z = 0.f, up = 0.f;
+      for (int r = 0; r < a.split; ++r) {
+        z += load_share(at, r);
+        if constexpr (GATED) up += load_share(at + TOK * BN * 4, r);
+      }
+      finish<T, GATED>(a, m0 + t, n0 + c, z, up);
+    }
+    __syncwarp();
+    cluster_sync();                    // nobody still reads this CTA's share
+  }
+}
+
+template <typename T, int TOK, bool GATED>
+std::string launch_tok(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw, int split,
+                       const LaunchCtx& ctx) {
+  using C = Config<TOK, GATED>;
+  const CUtensorMapDataType type =
+      p.elt == Elt::BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  Maps maps{};
+  std::string e = make_operand_map(&maps.x, type, p.x, p.M, p.K, lx, TOK);
+  if (e.empty()) e = make_operand_map(&maps.w, type, p.w, p.N, p.K, lw, BN);
+  if (e.empty() && p.x2) e = make_operand_map(&maps.x2, type, p.x2, p.M, p.K, lx, TOK);
+  if (e.empty() && p.w2) e = make_operand_map(&maps.w2, type, p.w2, p.N, p.K, lw, BN);
+  if (!e.empty()) return e;
+  Args a{};
+  a.M = (int)p.M; a.N = (int)p.N; a.K = (int)p.K;
+  a.act = (int)p.act;
+  a.sum = p.mode == LinearMode::Sum;
+  a.w_mn = lw.mn;
+  a.split = split;
+  a.bias = p.bias; a.residual = p.residual;
+  a.out = p.out; a.pre = p.pre; a.pre2 = p.pre2;
+  a.srm = p.srm; a.som = p.som; a.spm = p.spm;
+  auto kernel = linear_narrow_kernel<T, TOK, GATED>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (err != cudaSuccess) return cudaGetErrorString(err);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)((p.N + BN - 1) / BN * split), (unsigned)((p.M + TOK - 1) / TOK));
+  config.blockDim = dim3(NUM_THREADS);
+  config.dynamicSmemBytes = C::SMEM;
+  config.stream = ctx.stream;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = (unsigned)split;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  err = cudaLaunchKernelEx(&config, kernel, maps, a, ctx.status);
+  ++*ctx.launches;
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    return std::string("launch failed: ") + cudaGetErrorString(err);
+  }
+  return std::string();
+}
+
+template <typename T, bool GATED>
+std::string launch_rows(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw, const NarrowPlan& plan,
+                        const LaunchCtx& ctx) {
+  switch (plan.rows) {
+    case 16: return launch_tok<T, 16, GATED>(p, lx, lw, plan.split, ctx);
+    case 32: return launch_tok<T, 32, GATED>(p, lx, lw, plan.split, ctx);
+    case 64: return launch_tok<T, 64, GATED>(p, lx, lw, plan.split, ctx);
+    default: return launch_tok<T, 128, GATED>(p, lx, lw, plan.split, ctx);
+  }
+}
+
+}  // namespace
+
+bool plan_linear_narrow(const LinearProblem& p, const OperandLayout& lx, int sm_count, NarrowPlan* plan) {
+  if (lx.mn || p.mode == LinearMode::Pair) return false;
+  plan->rows = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+  const int64_t tiles = (p.N + BN - 1) / BN * ((p.M + plan->rows - 1) / plan->rows);
+  if ((p.M + plan->rows - 1) / plan->rows > 65535 || tiles > 0x0fffffff) return false;
+  const int64_t blocks = (p.K + BK - 1) / BK * (p.mode == LinearMode::Sum ? 2 : 1);
+  const int64_t slots = (int64_t)sm_count * (plan->rows <= 64 ? 2 : 1);
+  // the split whose last CTA is done first: waves of CTAs times k-blocks each, plus the exchange
+  double best = 0;
+  plan->split = 0;
+  const int per_block = (p.mode == LinearMode::Gated ? 2 : 1) * 16 + plan->rows / 8;      // KB of a k-block
+  for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
+    const int64_t ctas = tiles * split;
+    const int64_t each = (blocks + split - 1) / split;
+    // An SM takes in at most about 45 bytes a clock, all of them together 3400 (6.5 TB/s at 1.9 GHz).
+    const double alone = (double)std::min<int64_t>(ctas, sm_count) * 45.0;
+    const double rate = std::min(alone, 3400.0) / (double)std::min<int64_t>(ctas, slots);      // bytes a clock of a CTA
+    const int64_t waves = (ctas + slots - 1) / slots;
+    const double time = (double)waves * (double)each * per_block * 1024.0 / rate + (split > 1 ? 2000.0 : 0.0);
+    if (!plan->split || time < best) {
+      best = time;
+      plan->split = split;
+    }
+  }
+  plan->clocks = best + 6000.0;
+  return true;
+}
+
+std::string launch_linear_narrow(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw,
+                                 const NarrowPlan& plan, const LaunchCtx& ctx) {
+  const bool gated = p.mode == LinearMode::Gated;
+  if (p.elt == Elt::BF16)
+    return gated ? launch_rows<__nv_bfloat16, true>(p, lx, lw, plan, ctx)
+                 : launch_rows<__nv_bfloat16, false>(p, lx, lw, plan, ctx);
+  return gated ? launch_rows<__half, true>(p, lx, lw, plan, ctx) : launch_rows<__half, false>(p, lx, lw, plan, ctx);
+}
+
+}  // namespace tmc

@@ -432,23 +432,6 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
 
 // ---- host ----------------------------------------------------------------------------------------
 
-// The map of an operand with `outer` rows (m or n) of K elements: contiguous along k (`mn` = 0) or along
-// its rows' index (`mn` = 1).
-std::string operand_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t outer, int64_t K,
-                        const OperandLayout& l, int box_outer) {
-  uint64_t dims[2], strides[1];
-  uint32_t box[2];
-  if (!l.mn) {
-    dims[0] = (uint64_t)K; dims[1] = (uint64_t)outer;
-    box[0] = BK; box[1] = (uint32_t)box_outer;
-  } else {
-    dims[0] = (uint64_t)outer; dims[1] = (uint64_t)K;
-    box[0] = 64; box[1] = BK;
-  }
-  strides[0] = (uint64_t)l.stride * 2;
-  return make_tensor_map(map, type, 2, base, dims, strides, box);
-}
-
 std::string output_map(CUtensorMap* map, CUtensorMapDataType type, void* base, int64_t M, int64_t N,
                        int64_t stride) {
   uint64_t dims[2] = {(uint64_t)N, (uint64_t)M};
@@ -478,10 +461,10 @@ std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const O
   a.tma_pre = aligned(p.pre, p.spm) && aligned(p.pre2, p.spm);
   a.vec_bias = (uintptr_t)p.bias % 16 == 0;
   a.vec_residual = (uintptr_t)p.residual % 16 == 0 && p.srm % 8 == 0;
-  std::string e = operand_map(&maps.x, type, p.x, p.M, p.K, lx, BM);
-  if (e.empty()) e = operand_map(&maps.w, type, p.w, p.N, p.K, lw, BN / 2);
-  if (e.empty() && p.x2) e = operand_map(&maps.x2, type, p.x2, p.M, p.K, lx, BM);
-  if (e.empty() && p.w2) e = operand_map(&maps.w2, type, p.w2, p.N, p.K, lw, BN / 2);
+  std::string e = make_operand_map(&maps.x, type, p.x, p.M, p.K, lx, BM);
+  if (e.empty()) e = make_operand_map(&maps.w, type, p.w, p.N, p.K, lw, BN / 2);
+  if (e.empty() && p.x2) e = make_operand_map(&maps.x2, type, p.x2, p.M, p.K, lx, BM);
+  if (e.empty() && p.w2) e = make_operand_map(&maps.w2, type, p.w2, p.N, p.K, lw, BN / 2);
   if (e.empty() && a.tma_out) e = output_map(&maps.out, type, p.out, p.M, p.N, p.som);
   if (e.empty() && a.tma_out && p.out2) e = output_map(&maps.out2, type, p.out2, p.M, p.N, p.som);
   if (e.empty() && a.tma_pre && p.pre) e = output_map(&maps.pre, type, p.pre, p.M, p.N, p.spm);
@@ -507,6 +490,30 @@ std::string launch_typed(const LinearProblem& p, const OperandLayout& lx, const 
 }
 
 }  // namespace
+
+std::string make_operand_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t outer, int64_t K,
+                             const OperandLayout& l, int box_outer) {
+  uint64_t dims[2], strides[1];
+  uint32_t box[2];
+  if (!l.mn) {
+    dims[0] = (uint64_t)K; dims[1] = (uint64_t)outer;
+    box[0] = BK; box[1] = (uint32_t)box_outer;
+  } else {
+    dims[0] = (uint64_t)outer; dims[1] = (uint64_t)K;
+    box[0] = 64; box[1] = BK;
+  }
+  strides[0] = (uint64_t)l.stride * 2;
+  return make_tensor_map(map, type, 2, base, dims, strides, box);
+}
+
+double estimate_linear_tc(const LinearProblem& p, int sm_count) {
+  // a tile's k-block takes 512 clocks (256 x 256 x 64 on two SMs), its epilogue hides under the next tile
+  const int64_t cols = p.mode == LinearMode::Gated ? 128 : 256;
+  const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + cols - 1) / cols) * (p.mode == LinearMode::Pair ? 2 : 1);
+  const int64_t blocks = (p.K + BK - 1) / BK * (p.mode == LinearMode::Sum ? 2 : 1);
+  const int64_t waves = (tiles + sm_count / 2 - 1) / (sm_count / 2);
+  return (double)waves * ((double)blocks * 540.0) + 8000.0;
+}
 
 std::string launch_linear_tc(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw,
                              const LaunchCtx& ctx) {
