@@ -164,23 +164,24 @@ std::string launch_typed(const ActBwdProblem& p, const LaunchCtx& ctx) {
 struct SumOutputs {
   void* out[kMaxColumnSums];
 };
+// 32 columns and 32 shares of the rows a block: the rows come from L2, eight in flight a thread.
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ partial, int64_t parts,
-                                                          int64_t N, const SumOutputs outs) {
-  __shared__ float joined[8][33];
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float* __restrict__ partial, int64_t parts, int64_t N,
+                                                           const SumOutputs outs) {
+  __shared__ float joined[32][33];
   const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
   const int64_t n = (int64_t)blockIdx.x * 32 + tx;
   const float* base = partial + (int64_t)blockIdx.y * parts * N;
   float total = 0.f;
   if (n < N) {
 #pragma unroll 8
-    for (int64_t r = ty; r < parts; r += 8) total += base[r * N + n];
+    for (int64_t r = ty; r < parts; r += 32) total += base[r * N + n];
   }
   joined[ty][tx] = total;
   __syncthreads();
   if (ty == 0 && n < N) {
 #pragma unroll
-    for (int r = 1; r < 8; ++r) total += joined[r][tx];
+    for (int r = 1; r < 32; ++r) total += joined[r][tx];
     ((T*)outs.out[blockIdx.y])[n] = from_f32<T>(total);
   }
 }
@@ -192,9 +193,9 @@ void launch_column_sums(Elt elt, const float* partial, int64_t parts, int64_t N,
   SumOutputs outs{};
   for (int i = 0; i < sets; ++i) outs.out[i] = out[i];
   const dim3 grid((unsigned)((N + 31) / 32), (unsigned)sets);
-  if (elt == Elt::F32) column_sums_kernel<float><<<grid, 256, 0, ctx.stream>>>(partial, parts, N, outs);
-  else if (elt == Elt::BF16) column_sums_kernel<__nv_bfloat16><<<grid, 256, 0, ctx.stream>>>(partial, parts, N, outs);
-  else column_sums_kernel<__half><<<grid, 256, 0, ctx.stream>>>(partial, parts, N, outs);
+  if (elt == Elt::F32) column_sums_kernel<float><<<grid, 1024, 0, ctx.stream>>>(partial, parts, N, outs);
+  else if (elt == Elt::BF16) column_sums_kernel<__nv_bfloat16><<<grid, 1024, 0, ctx.stream>>>(partial, parts, N, outs);
+  else column_sums_kernel<__half><<<grid, 1024, 0, ctx.stream>>>(partial, parts, N, outs);
   ++*ctx.launches;
 }
 
