@@ -73,6 +73,9 @@ void launch_column_sums(Elt elt, const float* partial, int64_t parts, int64_t N,
 
 // Any strides, any alignment, fp32 accumulation on the CUDA cores.
 std::string launch_linear_simt(const LinearProblem& p, const LaunchCtx& ctx);
+// fp32 operands that are contiguous along one dimension.
+bool linear_f32_takes(const LinearProblem& p);
+std::string launch_linear_f32(const LinearProblem& p, const LaunchCtx& ctx);
 // Picks the kernel (path_option: 0 automatic, 1 the CUDA cores, 2 the tensor cores or `refused` says why
 // not) and reports which it was (1 or 2).
 std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path_option, int* path_used,

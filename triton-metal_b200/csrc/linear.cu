@@ -106,7 +106,7 @@ std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path
       *refused = why;
       return std::string();
     }
-    return launch_linear_simt(p, ctx);
+    return linear_f32_takes(p) ? launch_linear_f32(p, ctx) : launch_linear_simt(p, ctx);
   }
   *path_used = 2;
   if (x_fits && w_fits) return launch_tensor(p, lx, lw, ctx);

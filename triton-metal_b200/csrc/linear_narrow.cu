@@ -208,7 +208,6 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     ok = mbar_wait(smem_u32(&bars.acc_full), 0, wc, kEpiAccFull);
     tc_fence_after();
     const uint32_t lanes = tmem_base + ((uint32_t)(warp * 32) << 16);
-    const int n = n0 + warp * 32 + lane;
     float* share = reinterpret_cast<float*>(smem);       // [GATED][row][128 columns]: the ring is idle now
 #pragma unroll 1
     for (int t = 0; t < rows && __all_sync(0xffffffffu, ok); t += 16) {
@@ -219,13 +218,8 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         if (t + i >= rows) break;
-        const float v = __uint_as_float(z[i]), u = GATED ? __uint_as_float(up[i]) : 0.f;
-        if (a.split > 1) {
-          share[(t + i) * BN + warp * 32 + lane] = v;
-          if constexpr (GATED) share[(TOK + t + i) * BN + warp * 32 + lane] = u;
-        } else if (n < a.N) {
-          finish<T, GATED>(a, m0 + t + i, n, v, u);
-        }
+        share[(t + i) * BN + warp * 32 + lane] = __uint_as_float(z[i]);
+        if constexpr (GATED) share[(TOK + t + i) * BN + warp * 32 + lane] = __uint_as_float(up[i]);
       }
     }
   }
@@ -236,20 +230,28 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
-  if (a.split > 1) {
-    cluster_sync();                    // every share is written
-    const int width = BN / a.split;
-    for (int i = threadIdx.x; i < rows * width; i += NUM_THREADS) {
-      const int t = i / width, c = (int)rank * width + i % width;
-      if (n0 + c >= a.N) continue;
+  // (a rolled loop over the shares, also without a cluster: the activation's code appears once)
+  if (a.split > 1) cluster_sync();     // every share is written
+  const int width = BN / a.split;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < rows * width; i += NUM_THREADS) {
+    const int t = i / width, c = (int)rank * width + i % width;
+    if (n0 + c >= a.N) continue;
+    float z = 0.f, up = 0.f;
+    if (a.split > 1) {
       const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
-      float z = 0.f, up = 0.f;
       for (int r = 0; r < a.split; ++r) {
         z += load_share(at, r);
         if constexpr (GATED) up += load_share(at + TOK * BN * 4, r);
       }
-      finish<T, GATED>(a, m0 + t, n0 + c, z, up);
+    } else {
+      const float* share = reinterpret_cast<const float*>(smem);
+      z = share[t * BN + c];
+      if constexpr (GATED) up = share[(TOK + t) * BN + c];
     }
+    finish<T, GATED>(a, m0 + t, n0 + c, z, up);
+  }
+  if (a.split > 1) {
     __syncwarp();
     cluster_sync();                    // nobody still reads this CTA's share
   }
