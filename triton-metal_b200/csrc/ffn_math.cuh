@@ -64,12 +64,32 @@ constexpr float kInvSqrt2Pi = 0.39894228040143267794f;
 constexpr float kTanhA = 0.79788456080286535588f;   // sqrt(2 / pi)
 constexpr float kTanhB = 0.044715f;
 
+// The normal distribution's upper tail at |z|, 1 - Phi(|z|) = erfc(|z| / sqrt 2) / 2, for 16-bit results: the
+// rational approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions (absolute error
+// below 1.5e-7 of erf), fourteen instructions without a branch where erff takes both of its two.  `density`
+// is exp(-z^2 / 2), which the derivative needs too.
+__device__ __forceinline__ float normal_tail(float z, float& density) {
+  const float x = fabsf(z) * 0.70710678118654752440f;
+  density = __expf(-x * x);
+  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+  float poly = fmaf(1.061405429f, t, -1.453152027f);
+  poly = fmaf(poly, t, 1.421413741f);
+  poly = fmaf(poly, t, -0.284496736f);
+  poly = fmaf(poly, t, 0.254829592f);
+  return 0.5f * poly * t * density;
+}
+
 // gelu_tanh(z) = z/2 (1 + tanh(a(z + b z^3))) = z sigmoid(2a(z + b z^3)): no cancellation for z < 0.
 template <bool PRECISE>
 __device__ __forceinline__ float act_forward(Act act, float z) {
   switch (act) {
     case Act::Relu: return z != z ? z : fmaxf(z, 0.f);          // fmaxf alone would drop a NaN
-    case Act::Gelu: return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+    case Act::Gelu: {
+      if constexpr (PRECISE) return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+      float density;
+      const float tail = normal_tail(z, density);
+      return z * (z < 0.f ? tail : 1.f - tail);
+    }
     case Act::GeluTanh: return z * sigmoid<PRECISE>(2.f * kTanhA * (z + kTanhB * z * z * z));
     case Act::Silu: return z * sigmoid<PRECISE>(z);
     case Act::Sigmoid: return sigmoid<PRECISE>(z);
@@ -82,8 +102,10 @@ __device__ __forceinline__ float act_derivative(Act act, float z) {
   switch (act) {
     case Act::Relu: return z != z ? z : (z > 0.f ? 1.f : 0.f);
     case Act::Gelu: {
-      const float density = kInvSqrt2Pi * (PRECISE ? expf(-0.5f * z * z) : __expf(-0.5f * z * z));
-      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * density;
+      if constexpr (PRECISE) return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expf(-0.5f * z * z);
+      float density;
+      const float tail = normal_tail(z, density);
+      return fmaf(z * kInvSqrt2Pi, density, z < 0.f ? tail : 1.f - tail);
     }
     case Act::GeluTanh: {
       const float s = sigmoid<PRECISE>(2.f * kTanhA * (z + kTanhB * z * z * z));

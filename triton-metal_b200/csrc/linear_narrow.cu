@@ -65,7 +65,9 @@ struct Args {
   const void *bias, *residual;
   void *out, *pre, *pre2;
   int64_t srm, som, spm;
+  int quads;                           // kQuad...: every fourth element of the operand's rows is 8-byte aligned
 };
+enum : int { kQuadOut = 1, kQuadPre = 2, kQuadBias = 4, kQuadResidual = 8 };
 
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -76,27 +78,62 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float load_share(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ float4 load_share(uint32_t addr, uint32_t rank) {
   uint32_t remote;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote)
+               : "memory");
   return v;
 }
 
-template <typename T, bool GATED>
-__device__ __forceinline__ void finish(const Args& a, int m, int n, float z, float up) {
-  if constexpr (GATED) {
-    if (a.pre) ((T*)a.pre)[(int64_t)m * a.spm + n] = from_f32<T>(z);
-    if (a.pre2) ((T*)a.pre2)[(int64_t)m * a.spm + n] = from_f32<T>(up);
-    z = act_forward<false>((Act)a.act, z) * up;
+// Four neighbouring elements of an output or a bias / residual: one 8-byte access where the address allows.
+template <typename T>
+__device__ __forceinline__ void add4(float (&v)[4], const T* from, int left, bool quads) {
+  if (quads && left >= 4) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(from);
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += to_f32(e[i]);
   } else {
-    if (a.bias) z += to_f32(((const T*)a.bias)[n]);
-    if (a.pre) ((T*)a.pre)[(int64_t)m * a.spm + n] = from_f32<T>(z);
-    z = act_forward<false>((Act)a.act, z);
-    if (a.residual) z += to_f32(((const T*)a.residual)[(int64_t)m * a.srm + n]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) v[i] += to_f32(from[i]);
   }
-  ((T*)a.out)[(int64_t)m * a.som + n] = from_f32<T>(z);
+}
+template <typename T>
+__device__ __forceinline__ void put4(T* to, const float (&v)[4], int left, bool quads) {
+  if (quads && left >= 4) {
+    uint2 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<uint2*>(to) = raw;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) to[i] = from_f32<T>(v[i]);
+  }
+}
+
+// Outputs n ... n + 3 of row m (`left` of them exist) from x w, and from x w2 of a gated product.
+template <typename T, bool GATED>
+__device__ __forceinline__ void finish(const Args& a, int64_t m, int n, int left, float (&z)[4], float (&up)[4]) {
+  if constexpr (GATED) {
+    if (a.pre) put4((T*)a.pre + m * a.spm + n, z, left, a.quads & kQuadPre);
+    if (a.pre2) put4((T*)a.pre2 + m * a.spm + n, up, left, a.quads & kQuadPre);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>((Act)a.act, z[i]) * up[i];
+  } else {
+    if (a.bias) add4(z, (const T*)a.bias + n, left, a.quads & kQuadBias);
+    if (a.pre) put4((T*)a.pre + m * a.spm + n, z, left, a.quads & kQuadPre);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>((Act)a.act, z[i]);
+    if (a.residual) add4(z, (const T*)a.residual + m * a.srm + n, left, a.quads & kQuadResidual);
+  }
+  put4((T*)a.out + m * a.som + n, z, left, a.quads & kQuadOut);
 }
 
 template <typename T, int TOK, bool GATED>
@@ -110,7 +147,7 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
   Barriers& bars = *reinterpret_cast<Barriers*>(smem + STAGES * STAGE_BYTES);
   const uint32_t smem_base = smem_u32(smem);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t rank = a.split > 1 ? cta_rank() : 0;
+  const uint32_t rank = cta_rank();          // 0 without a cluster
   WaitCtx wc{&bars.abort_flag, status};
 
   const int n0 = (int)(blockIdx.x / a.split) * BN, m0 = (int)blockIdx.y * TOK;
@@ -119,7 +156,31 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
   const int blocks = a.sum ? 2 * blocks_one : blocks_one;
   const int kb0 = (int)((int64_t)blocks * rank / a.split), kb1 = (int)((int64_t)blocks * (rank + 1) / a.split);
 
-  if (threadIdx.x == 0) {
+  // One k-block of both operands into a slot of the ring.
+  auto fetch = [&](int kb, int stage) {
+    const bool other = kb >= blocks_one;                             // sum: the second pair of operands
+    const int k = (other ? kb - blocks_one : kb) * BK;
+    const uint32_t bar = smem_u32(&bars.full[stage]);
+    uint32_t dst = smem_base + stage * STAGE_BYTES;
+    mbar_expect_tx(bar, STAGE_BYTES);
+#pragma unroll
+    for (int g = 0; g < (GATED ? 2 : 1); ++g) {
+      const CUtensorMap* mw = g || other ? &maps.w2 : &maps.w;
+      if (a.w_mn) {
+        tma_load_2d(dst, mw, bar, n0, k);
+        tma_load_2d(dst + 8192, mw, bar, n0 + 64, k);
+      } else {
+        tma_load_2d(dst, mw, bar, k, n0);
+      }
+      dst += W_BYTES;
+    }
+    tma_load_2d(dst, other ? &maps.x2 : &maps.x, bar, k, m0);
+  };
+
+  // The thread that makes the barriers fills the ring at once: the first weights are under way while the
+  // TMEM is allocated and the other warps arrive.
+  const int ahead = min(STAGES, kb1 - kb0);
+  if (warp == 4 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&bars.full[s]), 1);
       mbar_init(smem_u32(&bars.empty[s]), 1);
@@ -127,15 +188,13 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     mbar_init(smem_u32(&bars.acc_full), 1);
     bars.abort_flag = 0;
     fence_barrier_init();
+    for (int s = 0; s < ahead; ++s) fetch(kb0 + s, s);
   }
   if (warp == 5) {
     tmem_alloc(smem_u32(&bars.tmem_base), C::TMEM_COLS);
     tmem_relinquish();
   }
-  if (warp == 4 && lane == 0) {
-    tma_prefetch_desc(&maps.x);
-    tma_prefetch_desc(&maps.w);
-  }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -145,27 +204,11 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
   if (warp == 4) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, issued = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      int stage = ahead == STAGES ? 0 : ahead;
+      uint32_t phase = ahead == STAGES ? 1 : 0, issued = ahead;
+      for (int kb = kb0 + ahead; kb < kb1; ++kb) {
         if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1, wc, kProdEmpty)) { ok = false; break; }
-        const bool other = kb >= blocks_one;                         // sum: the second pair of operands
-        const int k = (other ? kb - blocks_one : kb) * BK;
-        const uint32_t bar = smem_u32(&bars.full[stage]);
-        uint32_t dst = smem_base + stage * STAGE_BYTES;
-        mbar_expect_tx(bar, STAGE_BYTES);
-#pragma unroll
-        for (int g = 0; g < (GATED ? 2 : 1); ++g) {
-          const CUtensorMap* mw = g || other ? &maps.w2 : &maps.w;
-          if (a.w_mn) {
-            tma_load_2d(dst, mw, bar, n0, k);
-            tma_load_2d(dst + 8192, mw, bar, n0 + 64, k);
-          } else {
-            tma_load_2d(dst, mw, bar, k, n0);
-          }
-          dst += W_BYTES;
-        }
-        tma_load_2d(dst, other ? &maps.x2 : &maps.x, bar, k, m0);
+        fetch(kb, stage);
         ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
@@ -230,26 +273,32 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
-  // (a rolled loop over the shares, also without a cluster: the activation's code appears once)
+  // Four columns of a row at a time, the shares of the whole cluster loaded before the first is added.  (One
+  // loop for all cases, so that the activation's code appears once.)
   if (a.split > 1) cluster_sync();     // every share is written
-  const int width = BN / a.split;
+  const int width = BN / a.split, quads = width / 4;
 #pragma unroll 1
-  for (int i = threadIdx.x; i < rows * width; i += NUM_THREADS) {
-    const int t = i / width, c = (int)rank * width + i % width;
-    if (n0 + c >= a.N) continue;
-    float z = 0.f, up = 0.f;
-    if (a.split > 1) {
-      const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
-      for (int r = 0; r < a.split; ++r) {
-        z += load_share(at, r);
-        if constexpr (GATED) up += load_share(at + TOK * BN * 4, r);
-      }
-    } else {
-      const float* share = reinterpret_cast<const float*>(smem);
-      z = share[t * BN + c];
-      if constexpr (GATED) up = share[(TOK + t) * BN + c];
-    }
-    finish<T, GATED>(a, m0 + t, n0 + c, z, up);
+  for (int i = threadIdx.x; i < rows * quads; i += NUM_THREADS) {
+    const int t = i / quads, c = (int)rank * width + (i - t * quads) * 4;
+    const int left = a.N - n0 - c;
+    if (left <= 0) continue;
+    const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
+    float z[4], up[4] = {0.f, 0.f, 0.f, 0.f};
+    auto gather = [&](uint32_t addr, float (&sum)[4]) {
+      float4 part[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < a.split) part[r] = load_share(addr, r);
+      sum[0] = part[0].x; sum[1] = part[0].y; sum[2] = part[0].z; sum[3] = part[0].w;
+#pragma unroll
+      for (int r = 1; r < 8; ++r)
+        if (r < a.split) {
+          sum[0] += part[r].x; sum[1] += part[r].y; sum[2] += part[r].z; sum[3] += part[r].w;
+        }
+    };
+    gather(at, z);
+    if constexpr (GATED) gather(at + TOK * BN * 4, up);
+    finish<T, GATED>(a, m0 + t, n0 + c, left, z, up);
   }
   if (a.split > 1) {
     __syncwarp();
@@ -278,6 +327,11 @@ std::string launch_tok(const LinearProblem& p, const OperandLayout& lx, const Op
   a.bias = p.bias; a.residual = p.residual;
   a.out = p.out; a.pre = p.pre; a.pre2 = p.pre2;
   a.srm = p.srm; a.som = p.som; a.spm = p.spm;
+  auto quad = [&](const void* q, const void* q2, int64_t stride, int bit) {
+    return (((uintptr_t)q | (uintptr_t)q2) % 8 == 0 && (p.M <= 1 || stride % 4 == 0)) ? bit : 0;
+  };
+  a.quads = quad(p.out, nullptr, p.som, kQuadOut) | quad(p.pre, p.pre2, p.spm, kQuadPre) | quad(p.bias, nullptr, 0, kQuadBias) |
+            quad(p.residual, nullptr, p.srm, kQuadResidual);
   auto kernel = linear_narrow_kernel<T, TOK, GATED>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (err != cudaSuccess) return cudaGetErrorString(err);
@@ -328,8 +382,9 @@ bool plan_linear_narrow(const LinearProblem& p, const OperandLayout& lx, int sm_
   for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
     const int64_t ctas = tiles * split;
     const int64_t each = (blocks + split - 1) / split;
-    // An SM takes in at most about 45 bytes a clock, all of them together 3400 (6.5 TB/s at 1.9 GHz).
-    const double alone = (double)std::min<int64_t>(ctas, sm_count) * 45.0;
+    // An SM takes in about 36 bytes a clock (86 CTAs streamed 180 MB in 30 us), all of them together 3400
+    // (6.5 TB/s at 1.9 GHz).
+    const double alone = (double)std::min<int64_t>(ctas, sm_count) * 36.0;
     const double rate = std::min(alone, 3400.0) / (double)std::min<int64_t>(ctas, slots);      // bytes a clock of a CTA
     const int64_t waves = (ctas + slots - 1) / slots;
     const double time = (double)waves * (double)each * per_block * 1024.0 / rate + (split > 1 ? 2000.0 : 0.0);

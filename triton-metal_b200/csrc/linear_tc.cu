@@ -512,7 +512,10 @@ double estimate_linear_tc(const LinearProblem& p, int sm_count) {
   const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + cols - 1) / cols) * (p.mode == LinearMode::Pair ? 2 : 1);
   const int64_t blocks = (p.K + BK - 1) / BK * (p.mode == LinearMode::Sum ? 2 : 1);
   const int64_t waves = (tiles + sm_count / 2 - 1) / (sm_count / 2);
-  return (double)waves * ((double)blocks * 540.0) + 8000.0;
+  // With few rows it is bound by its operands' way from memory, at 2600 bytes a clock (it keeps fewer of them
+  // in flight than the kernel for few rows: 235 MB of gated weights took 49 us here, 41 us there).
+  const double bytes = 2.0 * ((double)p.K * (double)p.N * (p.w2 ? 2 : 1) + (double)p.M * (double)p.K);
+  return std::max((double)waves * ((double)blocks * 540.0), bytes / 2600.0) + 14000.0;
 }
 
 std::string launch_linear_tc(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw,
