@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(CX * RY) activation_bwd_kernel(const ActBwdPro
     with_act(p.act, [&](auto tag) {
       constexpr Act act = decltype(tag)::value;
       constexpr bool precise = sizeof(T) == 4;
-#pragma unroll 2
+#pragma unroll 4
       for (int64_t m = first + ty; m < last; m += RY) {
         float d[VEC];
         load_vec<T, VEC>((const T*)p.dout + m * p.s_dout + col, d);
@@ -164,26 +164,29 @@ std::string launch_typed(const ActBwdProblem& p, const LaunchCtx& ctx) {
 struct SumOutputs {
   void* out[kMaxColumnSums];
 };
-// 32 columns and 32 shares of the rows a block: the rows come from L2, eight in flight a thread.
+// 16 columns and 64 shares of the rows a block: the rows come from L2, eight in flight a thread, and a few
+// hundred of them are what the backward passes leave.
+constexpr int SUM_COLS = 16, SUM_ROWS = 64;
 template <typename T>
-__global__ void __launch_bounds__(1024) column_sums_kernel(const float* __restrict__ partial, int64_t parts, int64_t N,
-                                                           const SumOutputs outs) {
-  __shared__ float joined[32][33];
-  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-  const int64_t n = (int64_t)blockIdx.x * 32 + tx;
+__global__ void __launch_bounds__(SUM_COLS * SUM_ROWS) column_sums_kernel(const float* __restrict__ partial, int64_t parts,
+                                                                          int64_t N, const SumOutputs outs) {
+  __shared__ float joined[SUM_ROWS][SUM_COLS + 1];
+  const int tx = threadIdx.x % SUM_COLS, ty = threadIdx.x / SUM_COLS;
+  const int64_t n = (int64_t)blockIdx.x * SUM_COLS + tx;
   const float* base = partial + (int64_t)blockIdx.y * parts * N;
   float total = 0.f;
   if (n < N) {
 #pragma unroll 8
-    for (int64_t r = ty; r < parts; r += 32) total += base[r * N + n];
+    for (int64_t r = ty; r < parts; r += SUM_ROWS) total += base[r * N + n];
   }
   joined[ty][tx] = total;
   __syncthreads();
-  if (ty == 0 && n < N) {
 #pragma unroll
-    for (int r = 1; r < 32; ++r) total += joined[r][tx];
-    ((T*)outs.out[blockIdx.y])[n] = from_f32<T>(total);
+  for (int step = SUM_ROWS / 2; step > 0; step /= 2) {
+    if (ty < step) joined[ty][tx] += joined[ty + step][tx];
+    __syncthreads();
   }
+  if (ty == 0 && n < N) ((T*)outs.out[blockIdx.y])[n] = from_f32<T>(joined[0][tx]);
 }
 
 }  // namespace
@@ -192,10 +195,11 @@ void launch_column_sums(Elt elt, const float* partial, int64_t parts, int64_t N,
                         const LaunchCtx& ctx) {
   SumOutputs outs{};
   for (int i = 0; i < sets; ++i) outs.out[i] = out[i];
-  const dim3 grid((unsigned)((N + 31) / 32), (unsigned)sets);
-  if (elt == Elt::F32) column_sums_kernel<float><<<grid, 1024, 0, ctx.stream>>>(partial, parts, N, outs);
-  else if (elt == Elt::BF16) column_sums_kernel<__nv_bfloat16><<<grid, 1024, 0, ctx.stream>>>(partial, parts, N, outs);
-  else column_sums_kernel<__half><<<grid, 1024, 0, ctx.stream>>>(partial, parts, N, outs);
+  const dim3 grid((unsigned)((N + SUM_COLS - 1) / SUM_COLS), (unsigned)sets);
+  constexpr int THREADS = SUM_COLS * SUM_ROWS;
+  if (elt == Elt::F32) column_sums_kernel<float><<<grid, THREADS, 0, ctx.stream>>>(partial, parts, N, outs);
+  else if (elt == Elt::BF16) column_sums_kernel<__nv_bfloat16><<<grid, THREADS, 0, ctx.stream>>>(partial, parts, N, outs);
+  else column_sums_kernel<__half><<<grid, THREADS, 0, ctx.stream>>>(partial, parts, N, outs);
   ++*ctx.launches;
 }
 

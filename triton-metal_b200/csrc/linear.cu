@@ -42,20 +42,36 @@ struct CopyJob {
 struct CopyJobs {
   CopyJob job[4];
 };
+// Eight elements from any 2-byte aligned address, contiguous: five aligned words, shifted into place.
+__device__ __forceinline__ uint4 load_unaligned(const uint16_t* from) {
+  const uintptr_t at = (uintptr_t)from;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+  const uint32_t w0 = __ldg(words), w1 = __ldg(words + 1), w2 = __ldg(words + 2), w3 = __ldg(words + 3);
+  if (!(at & 2)) return make_uint4(w0, w1, w2, w3);
+  const uint32_t w4 = __ldg(reinterpret_cast<const uint16_t*>(words + 4));    // only its lower half is ours
+  return make_uint4(__funnelshift_r(w0, w1, 16), __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16),
+                    __funnelshift_r(w3, w4, 16));
+}
 __global__ void __launch_bounds__(256) align_operands_kernel(const CopyJobs jobs) {
   const CopyJob& j = jobs.job[blockIdx.y];
   const int64_t packets = j.pitch / 8, total = j.rows * packets;
+#pragma unroll 2
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / packets, c = (i - r * packets) * 8;
     const uint16_t* from = j.from + r * j.row_stride + c * j.col_stride;
-    uint16_t e[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) e[k] = c + k < j.cols ? from[k * j.col_stride] : (uint16_t)0;
     uint4 v;
-    v.x = e[0] | (uint32_t)e[1] << 16;
-    v.y = e[2] | (uint32_t)e[3] << 16;
-    v.z = e[4] | (uint32_t)e[5] << 16;
-    v.w = e[6] | (uint32_t)e[7] << 16;
+    // (a packet's first word may begin two bytes early: at the operand's own first element that is not ours)
+    if (j.col_stride == 1 && c + 8 <= j.cols && i > 0) {
+      v = load_unaligned(from);
+    } else {
+      uint16_t e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = c + k < j.cols ? from[k * j.col_stride] : (uint16_t)0;
+      v.x = e[0] | (uint32_t)e[1] << 16;
+      v.y = e[2] | (uint32_t)e[3] << 16;
+      v.z = e[4] | (uint32_t)e[5] << 16;
+      v.w = e[6] | (uint32_t)e[7] << 16;
+    }
     *reinterpret_cast<uint4*>(j.to + r * j.pitch + c) = v;
   }
 }

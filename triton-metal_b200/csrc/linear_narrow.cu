@@ -89,6 +89,10 @@ __device__ __forceinline__ float4 load_share(uint32_t addr, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ void add(float4& a, const float4& b) {
+  a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+}
+
 // Four neighbouring elements of an output or a bias / residual: one 8-byte access where the address allows.
 template <typename T>
 __device__ __forceinline__ void add4(float (&v)[4], const T* from, int left, bool quads) {
@@ -119,18 +123,20 @@ __device__ __forceinline__ void put4(T* to, const float (&v)[4], int left, bool 
 }
 
 // Outputs n ... n + 3 of row m (`left` of them exist) from x w, and from x w2 of a gated product.
-template <typename T, bool GATED>
-__device__ __forceinline__ void finish(const Args& a, int64_t m, int n, int left, float (&z)[4], float (&up)[4]) {
+template <typename T, bool GATED, Act ACT>
+__device__ __forceinline__ void finish(const Args& a, int64_t m, int n, int left, float4 sum, float4 sum2) {
+  float z[4] = {sum.x, sum.y, sum.z, sum.w};
   if constexpr (GATED) {
+    const float up[4] = {sum2.x, sum2.y, sum2.z, sum2.w};
     if (a.pre) put4((T*)a.pre + m * a.spm + n, z, left, a.quads & kQuadPre);
     if (a.pre2) put4((T*)a.pre2 + m * a.spm + n, up, left, a.quads & kQuadPre);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>((Act)a.act, z[i]) * up[i];
+    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>(ACT, z[i]) * up[i];
   } else {
     if (a.bias) add4(z, (const T*)a.bias + n, left, a.quads & kQuadBias);
     if (a.pre) put4((T*)a.pre + m * a.spm + n, z, left, a.quads & kQuadPre);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>((Act)a.act, z[i]);
+    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>(ACT, z[i]);
     if (a.residual) add4(z, (const T*)a.residual + m * a.srm + n, left, a.quads & kQuadResidual);
   }
   put4((T*)a.out + m * a.som + n, z, left, a.quads & kQuadOut);
@@ -273,33 +279,49 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
-  // Four columns of a row at a time, the shares of the whole cluster loaded before the first is added.  (One
-  // loop for all cases, so that the activation's code appears once.)
+  // Four columns of a row at a time, four such pieces a thread and turn: the shares of the whole cluster are
+  // loaded for all of them before the first is added, since each load takes hundreds of clocks.
   if (a.split > 1) cluster_sync();     // every share is written
-  const int width = BN / a.split, quads = width / 4;
+  const int width = BN / a.split, quads = width / 4, items = rows * quads;
+  with_act((Act)a.act, [&](auto tag) {
 #pragma unroll 1
-  for (int i = threadIdx.x; i < rows * quads; i += NUM_THREADS) {
-    const int t = i / quads, c = (int)rank * width + (i - t * quads) * 4;
-    const int left = a.N - n0 - c;
-    if (left <= 0) continue;
-    const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
-    float z[4], up[4] = {0.f, 0.f, 0.f, 0.f};
-    auto gather = [&](uint32_t addr, float (&sum)[4]) {
-      float4 part[8];
+    for (int base = threadIdx.x; base < items; base += 4 * NUM_THREADS) {
+      float4 z[4], up[4];
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < a.split) part[r] = load_share(addr, r);
-      sum[0] = part[0].x; sum[1] = part[0].y; sum[2] = part[0].z; sum[3] = part[0].w;
-#pragma unroll
-      for (int r = 1; r < 8; ++r)
-        if (r < a.split) {
-          sum[0] += part[r].x; sum[1] += part[r].y; sum[2] += part[r].z; sum[3] += part[r].w;
+      for (int q = 0; q < 4; ++q) {
+        const int i = min(base + q * NUM_THREADS, items - 1), t = i / quads, c = (int)rank * width + (i - t * quads) * 4;
+        const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
+        if (a.split == 1) {
+          z[q] = *reinterpret_cast<const float4*>(smem + (t * BN + c) * 4);
+          if constexpr (GATED) up[q] = *reinterpret_cast<const float4*>(smem + ((TOK + t) * BN + c) * 4);
+        } else {
+          z[q] = load_share(at, 0);
+          if constexpr (GATED) up[q] = load_share(at + TOK * BN * 4, 0);
         }
-    };
-    gather(at, z);
-    if constexpr (GATED) gather(at + TOK * BN * 4, up);
-    finish<T, GATED>(a, m0 + t, n0 + c, left, z, up);
-  }
+      }
+      for (int r = 1; r < a.split; ++r) {
+        float4 other[4], other_up[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = min(base + q * NUM_THREADS, items - 1), t = i / quads, c = (int)rank * width + (i - t * quads) * 4;
+          const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
+          other[q] = load_share(at, r);
+          if constexpr (GATED) other_up[q] = load_share(at + TOK * BN * 4, r);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          add(z[q], other[q]);
+          if constexpr (GATED) add(up[q], other_up[q]);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = base + q * NUM_THREADS, t = i / quads, c = (int)rank * width + (i - t * quads) * 4;
+        const int left = a.N - n0 - c;
+        if (i < items && left > 0) finish<T, GATED, decltype(tag)::value>(a, m0 + t, n0 + c, left, z[q], up[q]);
+      }
+    }
+  });
   if (a.split > 1) {
     __syncwarp();
     cluster_sync();                    // nobody still reads this CTA's share
@@ -387,7 +409,10 @@ bool plan_linear_narrow(const LinearProblem& p, const OperandLayout& lx, int sm_
     const double alone = (double)std::min<int64_t>(ctas, sm_count) * 36.0;
     const double rate = std::min(alone, 3400.0) / (double)std::min<int64_t>(ctas, slots);      // bytes a clock of a CTA
     const int64_t waves = (ctas + slots - 1) / slots;
-    const double time = (double)waves * (double)each * per_block * 1024.0 / rate + (split > 1 ? 2000.0 : 0.0);
+    // its rows of the sums, 768 groups of four columns a turn
+    const double rows = (double)std::min<int64_t>(plan->rows, p.M);
+    const double finish = (split > 1 ? 2000.0 : 0.0) + rows * (32.0 / split) / (4 * NUM_THREADS) * (split > 1 ? 1500.0 : 1000.0);
+    const double time = (double)waves * ((double)each * per_block * 1024.0 / rate + finish);
     if (!plan->split || time < best) {
       best = time;
       plan->split = split;

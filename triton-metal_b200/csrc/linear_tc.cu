@@ -43,10 +43,11 @@ constexpr int TMEM_COLS = 512;
 constexpr int BOX = 32 * 128;          // one warp's staged piece: 32 rows x 64 columns
 constexpr int A_BYTES = BM * BK * 2;
 
-template <int BN> struct Config {
-  static constexpr int B_BYTES = BN / 2 * BK * 2;         // this CTA's half of the w tile
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 6 : 7;
+// A tile is HALVES accumulators of BN columns side by side.
+template <int BN, int HALVES> struct Config {
+  static constexpr int B_BYTES = BN / 2 * BK * 2;         // this CTA's part of one accumulator's w columns
+  static constexpr int STAGE_BYTES = A_BYTES + HALVES * B_BYTES;
+  static constexpr int STAGES = HALVES == 2 ? 4 : BN == 256 ? 6 : 7;
   static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * BOX + 2048;
 };
 
@@ -212,13 +213,13 @@ __device__ __forceinline__ void load_tmem(uint32_t addr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-template <typename T, bool GATED, int BN>
+template <typename T, bool GATED, int BN, int HALVES>
 __global__ void __launch_bounds__(NUM_THREADS, 1) __cluster_dims__(2, 1, 1)
 linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a, DeviceStatus* status) {
-  using C = Config<BN>;
+  using C = Config<BN, HALVES>;
   constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES;
   constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-  constexpr int COLS = GATED ? BN / 2 : BN;           // output columns of a tile
+  constexpr int COLS = GATED ? BN / 2 : BN;           // output columns of an accumulator
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   Barriers& bars = *reinterpret_cast<Barriers*>(smem + STAGES * STAGE_BYTES + EPI_WARPS * BOX);
@@ -228,7 +229,7 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
   WaitCtx wc{&bars.abort_flag, status};
 
   const int tiles_m = (a.M + 2 * BM - 1) / (2 * BM);
-  const int tiles_one = (a.N + COLS - 1) / COLS;
+  const int tiles_one = (a.N + HALVES * COLS - 1) / (HALVES * COLS);
   const int tiles_n = a.mode == (int)LinearMode::Pair ? 2 * tiles_one : tiles_one;
   const int num_tiles = tiles_m * tiles_n;
   const int blocks_one = (a.K + BK - 1) / BK;
@@ -266,7 +267,7 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
         const bool second = tn >= tiles_one;                       // pair: the second product
         if (second) tn -= tiles_one;
         const int row = (tm * 2 + (int)rank) * BM;
-        const int col = GATED ? tn * COLS : tn * BN + (int)rank * (BN / 2);
+        const int col = tn * HALVES * COLS + (GATED ? 0 : (int)rank * (BN / 2));
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1, wc, kProdEmpty)) { ok = false; break; }
           const bool other = second || kb >= blocks_one;           // sum: the second pair of operands
@@ -282,11 +283,15 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
           } else {
             tma_load_pair(dst, mx, bar, k, row);
           }
-          if (a.w_mn) {
 #pragma unroll
-            for (int b = 0; b < BN / 128; ++b) tma_load_pair(dst + A_BYTES + b * 8192, mw, bar, col + b * 64, k);
-          } else {
-            tma_load_pair(dst + A_BYTES, mw, bar, k, col);
+          for (int h = 0; h < HALVES; ++h) {
+            const uint32_t to = dst + A_BYTES + h * C::B_BYTES;
+            if (a.w_mn) {
+#pragma unroll
+              for (int b = 0; b < BN / 128; ++b) tma_load_pair(to + b * 8192, mw, bar, col + h * COLS + b * 64, k);
+            } else {
+              tma_load_pair(to, mw, bar, k, col + h * COLS);
+            }
           }
           ++issued;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -324,23 +329,57 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-        const int acc = local & 1;
-        if (!mbar_wait_warp(smem_u32(&bars.acc_empty[acc]), ((local >> 1) & 1) ^ 1, wc, kMmaAccEmpty)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * 256;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait_warp(smem_u32(&bars.full[stage]), phase, wc, kMmaFull)) { ok = false; break; }
-          tc_fence_after();
-          const SmemDesc a_desc = a_base.advanced(stage * STAGE_BYTES);
-          const SmemDesc b_desc = b_base.advanced(stage * STAGE_BYTES);
+      auto products = [&](int at, int half, int acc, bool first_block) {
+        const SmemDesc a_desc = a_base.advanced(at * STAGE_BYTES);
+        const SmemDesc b_desc = b_base.advanced(at * STAGE_BYTES + half * C::B_BYTES);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            mma_pair_elect(d_tmem, a_desc.at(k * a_step), b_desc.at(k * b_step), idesc, (kb | k) != 0);
-          commit_pair_elect(smem_u32(&bars.empty[stage]));
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        for (int k = 0; k < BK / 16; ++k)
+          mma_pair_elect(tmem_base + acc * 256, a_desc.at(k * a_step), b_desc.at(k * b_step), idesc, !first_block || k != 0);
+      };
+      for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
+        if constexpr (HALVES == 1) {
+          const int acc = local & 1;
+          if (!mbar_wait_warp(smem_u32(&bars.acc_empty[acc]), ((local >> 1) & 1) ^ 1, wc, kMmaAccEmpty)) { ok = false; break; }
+          tc_fence_after();
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            if (!mbar_wait_warp(smem_u32(&bars.full[stage]), phase, wc, kMmaFull)) { ok = false; break; }
+            tc_fence_after();
+            products(stage, 0, acc, kb == 0);
+            commit_pair_elect(smem_u32(&bars.empty[stage]));
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+          if (ok) commit_pair_elect(smem_u32(&bars.acc_full[acc]));
+        } else {
+          // Both accumulators are still being read when the tile's operands are there: the first k-blocks go
+          // into the first half as soon as that is free, and catch up with the second when it is.
+          const int lead = min(STAGES, k_blocks);
+          int at = stage;
+          uint32_t ph = phase;
+          if (!mbar_wait_warp(smem_u32(&bars.acc_empty[0]), (local & 1) ^ 1, wc, kMmaAccEmpty)) { ok = false; break; }
+          tc_fence_after();
+          for (int kb = 0; kb < lead; ++kb) {
+            if (!mbar_wait_warp(smem_u32(&bars.full[at]), ph, wc, kMmaFull)) { ok = false; break; }
+            tc_fence_after();
+            products(at, 0, 0, kb == 0);
+            if (++at == STAGES) { at = 0; ph ^= 1; }
+          }
+          if (!ok) break;
+          if (lead == k_blocks) commit_pair_elect(smem_u32(&bars.acc_full[0]));
+          if (!mbar_wait_warp(smem_u32(&bars.acc_empty[1]), (local & 1) ^ 1, wc, kMmaAccEmpty)) { ok = false; break; }
+          tc_fence_after();
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            if (kb >= lead) {
+              if (!mbar_wait_warp(smem_u32(&bars.full[stage]), phase, wc, kMmaFull)) { ok = false; break; }
+              tc_fence_after();
+              products(stage, 0, 0, false);
+              if (kb == k_blocks - 1) commit_pair_elect(smem_u32(&bars.acc_full[0]));
+            }
+            products(stage, 1, 1, kb == 0);
+            commit_pair_elect(smem_u32(&bars.empty[stage]));
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+          if (ok) commit_pair_elect(smem_u32(&bars.acc_full[1]));
         }
-        if (ok) commit_pair_elect(smem_u32(&bars.acc_full[acc]));
       }
     }
   } else {
@@ -356,10 +395,6 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
       tile_coords(tile, tiles_m, tiles_n, a.group_m, tm, tn);
       const bool second = tn >= tiles_one;
       if (second) tn -= tiles_one;
-      const int acc = local & 1;
-      if (!mbar_wait(smem_u32(&bars.acc_full[acc]), (local >> 1) & 1, wc, kEpiAccFull)) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
       const int row0 = (tm * 2 + (int)rank) * BM + quarter * 32;
       const int row = row0 + lane;
       // out of a warp's registers into one of the outputs
@@ -379,44 +414,60 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
         staged = tma;
       };
 #pragma unroll 1
-      for (int c = part * 64; c < COLS && row0 < a.M; c += 128) {
-        // one piece: 64 output columns
-        const int col0 = tn * COLS + c;
-        if (col0 >= a.N) break;
-        float v[2][32];
-        load_tmem(lanes + c, v[0]);
-        load_tmem(lanes + c + 32, v[1]);
-        if constexpr (GATED) {
-          float up[2][32];
-          load_tmem(lanes + BN / 2 + c, up[0]);
-          load_tmem(lanes + BN / 2 + c + 32, up[1]);
-          if (a.pre) emit(&maps.pre, a.tma_pre, a.pre, a.spm, col0, v);
-          if (a.pre2) emit(&maps.pre2, a.tma_pre, a.pre2, a.spm, col0, up);
-          with_act(act, [&](auto tag) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[h][i] = act_forward<false>(decltype(tag)::value, v[h][i]) * up[h][i];
-          });
-        } else {
-          if (a.bias) add_row<T>(v, (const T*)a.bias + col0, a.N - col0, a.vec_bias);
-          if (a.pre) emit(&maps.pre, a.tma_pre, a.pre, a.spm, col0, v);
-          if (act != Act::None)
+      for (int half = 0; half < HALVES; ++half) {
+        const int acc = HALVES == 2 ? half : local & 1;
+        const uint32_t turn = HALVES == 2 ? local & 1 : (local >> 1) & 1;
+        if (!mbar_wait(smem_u32(&bars.acc_full[acc]), turn, wc, kEpiAccFull)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
+        const int first_col = (tn * HALVES + half) * COLS;
+        // the accumulator may be overwritten: tell the leader, from both CTAs
+        bool released = false;
+        auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(map_to_cta(smem_u32(&bars.acc_empty[acc]), 0));
+          released = true;
+        };
+#pragma unroll 1
+        for (int c = part * 64; c < COLS && row0 < a.M && first_col + c < a.N; c += 128) {
+          // one piece: 64 output columns
+          const int col0 = first_col + c;
+          const bool last = c + 128 >= COLS || col0 + 128 >= a.N;
+          float v[2][32];
+          load_tmem(lanes + c, v[0]);
+          load_tmem(lanes + c + 32, v[1]);
+          if constexpr (GATED) {
+            float up[2][32];
+            load_tmem(lanes + BN / 2 + c, up[0]);
+            load_tmem(lanes + BN / 2 + c + 32, up[1]);
+            if (last) release();
+            if (a.pre) emit(&maps.pre, a.tma_pre, a.pre, a.spm, col0, v);
+            if (a.pre2) emit(&maps.pre2, a.tma_pre, a.pre2, a.spm, col0, up);
             with_act(act, [&](auto tag) {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[h][i] = act_forward<false>(decltype(tag)::value, v[h][i]);
+                for (int i = 0; i < 32; ++i) v[h][i] = act_forward<false>(decltype(tag)::value, v[h][i]) * up[h][i];
             });
-          if (a.residual && row < a.M)
-            add_row<T>(v, (const T*)a.residual + (int64_t)row * a.srm + col0, a.N - col0, a.vec_residual);
+          } else {
+            if (last) release();
+            if (a.bias) add_row<T>(v, (const T*)a.bias + col0, a.N - col0, a.vec_bias);
+            if (a.pre) emit(&maps.pre, a.tma_pre, a.pre, a.spm, col0, v);
+            if (act != Act::None)
+              with_act(act, [&](auto tag) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) v[h][i] = act_forward<false>(decltype(tag)::value, v[h][i]);
+              });
+            if (a.residual && row < a.M)
+              add_row<T>(v, (const T*)a.residual + (int64_t)row * a.srm + col0, a.N - col0, a.vec_residual);
+          }
+          emit(second ? &maps.out2 : &maps.out, a.tma_out, second ? a.out2 : a.out, a.som, col0, v);
         }
-        emit(second ? &maps.out2 : &maps.out, a.tma_out, second ? a.out2 : a.out, a.som, col0, v);
+        if (!released) release();
       }
-      // the accumulator may be overwritten: tell the leader, from both CTAs
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_at(map_to_cta(smem_u32(&bars.acc_empty[acc]), 0));
     }
     if (lane == 0) tma_store_wait_all();
   }
@@ -440,9 +491,9 @@ std::string output_map(CUtensorMap* map, CUtensorMapDataType type, void* base, i
   return make_tensor_map(map, type, 2, base, dims, strides, box);
 }
 
-template <typename T, bool GATED, int BN>
+template <typename T, bool GATED, int BN, int HALVES>
 std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw, const LaunchCtx& ctx) {
-  using C = Config<BN>;
+  using C = Config<BN, HALVES>;
   constexpr int COLS = GATED ? BN / 2 : BN;
   const CUtensorMapDataType type =
       p.elt == Elt::BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -455,7 +506,7 @@ std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const O
   a.bias = p.bias; a.residual = p.residual;
   a.out = p.out; a.out2 = p.out2; a.pre = p.pre; a.pre2 = p.pre2;
   a.srm = p.srm; a.som = p.som; a.spm = p.spm;
-  a.group_m = 8;
+  a.group_m = 8;                     // row blocks (of 256) walked together: 4, 16 and 32 were 2 to 7 % slower
   auto aligned = [&](const void* q, int64_t stride) { return (uintptr_t)q % 16 == 0 && (p.M <= 1 || stride % 8 == 0); };
   a.tma_out = aligned(p.out, p.som) && aligned(p.out2, p.som);
   a.tma_pre = aligned(p.pre, p.spm) && aligned(p.pre2, p.spm);
@@ -470,10 +521,10 @@ std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const O
   if (e.empty() && a.tma_pre && p.pre) e = output_map(&maps.pre, type, p.pre, p.M, p.N, p.spm);
   if (e.empty() && a.tma_pre && p.pre2) e = output_map(&maps.pre2, type, p.pre2, p.M, p.N, p.spm);
   if (!e.empty()) return e;
-  auto kernel = linear_tc_kernel<T, GATED, BN>;
+  auto kernel = linear_tc_kernel<T, GATED, BN, HALVES>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (err != cudaSuccess) return cudaGetErrorString(err);
-  const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + COLS - 1) / COLS) * (p.mode == LinearMode::Pair ? 2 : 1);
+  const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + HALVES * COLS - 1) / (HALVES * COLS)) * (p.mode == LinearMode::Pair ? 2 : 1);
   if (tiles > 0x3fffffff) return "too many tiles";
   const int64_t pairs = std::min<int64_t>(tiles, ctx.sm_count / 2);
   kernel<<<(unsigned)(2 * pairs), NUM_THREADS, C::SMEM, ctx.stream>>>(maps, a, ctx.status);
@@ -483,10 +534,39 @@ std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const O
   return std::string();
 }
 
+// Clocks of a launch with tiles of 256 x `width` accumulator columns.  What an SM takes in bounds the narrower
+// ones: about 56 bytes a clock, against the 64 that a 256-column k-block's 512 clocks of products ask for (96 of
+// a 128-column one, 48 of a 512-column one).  The widest leaves no second accumulator, so half of its epilogue is
+// not hidden under the next tile's products.
+double tile_clocks(const LinearProblem& p, int width, int sm_count) {
+  const int64_t cols = p.mode == LinearMode::Gated ? width / 2 : width;
+  const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + cols - 1) / cols) * (p.mode == LinearMode::Pair ? 2 : 1);
+  const int64_t blocks = (p.K + BK - 1) / BK * (p.mode == LinearMode::Sum ? 2 : 1);
+  const int64_t waves = (tiles + sm_count / 2 - 1) / (sm_count / 2);
+  const bool light = p.act == Act::None && p.mode != LinearMode::Gated && !p.pre && !p.residual;
+  const double block = width == 512 ? 1040.0 : width == 256 ? 570.0 : 430.0;
+  return (double)waves * ((double)blocks * block + (width == 512 ? (light ? 2000.0 : 6000.0) : 300.0));
+}
+// The width that is done first.
+int tile_width(const LinearProblem& p, int sm_count) {
+  int best = 256;
+  for (int width : {128, 512})
+    if (tile_clocks(p, width, sm_count) < tile_clocks(p, best, sm_count)) best = width;
+  return best;
+}
+
+template <typename T, bool GATED>
+std::string launch_width(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw, const LaunchCtx& ctx) {
+  switch (tile_width(p, ctx.sm_count)) {
+    case 128: return launch_tile<T, GATED, 128, 1>(p, lx, lw, ctx);
+    case 256: return launch_tile<T, GATED, 256, 1>(p, lx, lw, ctx);
+    default: return launch_tile<T, GATED, 256, 2>(p, lx, lw, ctx);
+  }
+}
+
 template <typename T>
 std::string launch_typed(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw, const LaunchCtx& ctx) {
-  const bool gated = p.mode == LinearMode::Gated;
-  return gated ? launch_tile<T, true, 256>(p, lx, lw, ctx) : launch_tile<T, false, 256>(p, lx, lw, ctx);
+  return p.mode == LinearMode::Gated ? launch_width<T, true>(p, lx, lw, ctx) : launch_width<T, false>(p, lx, lw, ctx);
 }
 
 }  // namespace
@@ -507,15 +587,11 @@ std::string make_operand_map(CUtensorMap* map, CUtensorMapDataType type, const v
 }
 
 double estimate_linear_tc(const LinearProblem& p, int sm_count) {
-  // a tile's k-block takes 512 clocks (256 x 256 x 64 on two SMs), its epilogue hides under the next tile
-  const int64_t cols = p.mode == LinearMode::Gated ? 128 : 256;
-  const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + cols - 1) / cols) * (p.mode == LinearMode::Pair ? 2 : 1);
-  const int64_t blocks = (p.K + BK - 1) / BK * (p.mode == LinearMode::Sum ? 2 : 1);
-  const int64_t waves = (tiles + sm_count / 2 - 1) / (sm_count / 2);
   // With few rows it is bound by its operands' way from memory, at 2600 bytes a clock (it keeps fewer of them
   // in flight than the kernel for few rows: 235 MB of gated weights took 49 us here, 41 us there).
   const double bytes = 2.0 * ((double)p.K * (double)p.N * (p.w2 ? 2 : 1) + (double)p.M * (double)p.K);
-  return std::max((double)waves * ((double)blocks * 540.0), bytes / 2600.0) + 14000.0;
+  const double products = tile_clocks(p, tile_width(p, sm_count), sm_count);
+  return std::max(products, bytes / 2600.0) + 14000.0;
 }
 
 std::string launch_linear_tc(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw,
