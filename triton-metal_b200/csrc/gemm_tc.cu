@@ -66,7 +66,7 @@ static EncodeTiledFn encode_tiled_fn() {
 
 std::string make_tensor_map(CUtensorMap* out, CUtensorMapDataType type, int rank, const void* base,
                             const uint64_t* dims, const uint64_t* strides_bytes,
-                            const uint32_t* box) {
+                            const uint32_t* box, int swizzle_bytes) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return "cuTensorMapEncodeTiled is not available from this driver";
   cuuint64_t gdim[5];
@@ -80,7 +80,8 @@ std::string make_tensor_map(CUtensorMap* out, CUtensorMapDataType type, int rank
     if (i > 0) gstride[i - 1] = strides_bytes[i - 1];
   }
   CUresult r = fn(out, type, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstride, bdim, estride,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r);
   return std::string();

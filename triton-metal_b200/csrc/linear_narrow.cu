@@ -282,14 +282,14 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
   // Four columns of a row at a time, four such pieces a thread and turn: the shares of the whole cluster are
   // loaded for all of them before the first is added, since each load takes hundreds of clocks.
   if (a.split > 1) cluster_sync();     // every share is written
-  const int width = BN / a.split, quads = width / 4, items = rows * quads;
+  const int width = BN / a.split, shift = 31 - __clz(width / 4), items = rows << shift;
   with_act((Act)a.act, [&](auto tag) {
 #pragma unroll 1
     for (int base = threadIdx.x; base < items; base += 4 * NUM_THREADS) {
       float4 z[4], up[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int i = min(base + q * NUM_THREADS, items - 1), t = i / quads, c = (int)rank * width + (i - t * quads) * 4;
+        const int i = min(base + q * NUM_THREADS, items - 1), t = i >> shift, c = (int)rank * width + (i - (t << shift)) * 4;
         const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
         if (a.split == 1) {
           z[q] = *reinterpret_cast<const float4*>(smem + (t * BN + c) * 4);
@@ -303,7 +303,7 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
         float4 other[4], other_up[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int i = min(base + q * NUM_THREADS, items - 1), t = i / quads, c = (int)rank * width + (i - t * quads) * 4;
+          const int i = min(base + q * NUM_THREADS, items - 1), t = i >> shift, c = (int)rank * width + (i - (t << shift)) * 4;
           const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
           other[q] = load_share(at, r);
           if constexpr (GATED) other_up[q] = load_share(at + TOK * BN * 4, r);
@@ -316,7 +316,7 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int i = base + q * NUM_THREADS, t = i / quads, c = (int)rank * width + (i - t * quads) * 4;
+        const int i = base + q * NUM_THREADS, t = i >> shift, c = (int)rank * width + (i - (t << shift)) * 4;
         const int left = a.N - n0 - c;
         if (i < items && left > 0) finish<T, GATED, decltype(tag)::value>(a, m0 + t, n0 + c, left, z[q], up[q]);
       }

@@ -12,12 +12,13 @@
 // where both are registers of one thread.  The sum runs one K loop over both operand pairs; the pair
 // walks the columns of both results as one wider matrix, so that a shared x panel stays in L2.
 //
-//   warp 8   TMA producer (one lane): 64-deep k-blocks into a ring; both CTAs' loads complete on the
+//   warp 16  TMA producer (one lane): 64-deep k-blocks into a ring; both CTAs' loads complete on the
 //            leader's barrier
-//   warp 9   of the leader: tcgen05.mma 256 x BN x 16 into one of two TMEM accumulators; its commits
+//   warp 17  of the leader: tcgen05.mma 256 x BN x 16 into one of two TMEM accumulators; its commits
 //            release the ring slots and publish the accumulators in both CTAs
-//   warps 0-7  epilogue, thread = row, two warps per 32 rows: bias, activation, residual, rounding;
-//            64-column pieces leave through shared memory and TMA stores (clipped at the edges by the
+//   warps 0-15  epilogue, thread = row, four warps per 32 rows (with two, the activations' latencies kept a
+//            K = 1024 gelu tile at 841 TFLOP/s): bias, activation, residual, rounding;
+//            32-column pieces leave through shared memory and TMA stores (clipped at the edges by the
 //            tensor map), or, where the output's rows are not 16-byte aligned, as coalesced elements
 //
 // Either operand may be contiguous along k or along its other dimension (the descriptors say which), so
@@ -37,10 +38,10 @@ using namespace ffn;
 
 constexpr int BM = 128;                // rows of one CTA; a pair owns 256
 constexpr int BK = 64;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
 constexpr int NUM_THREADS = (EPI_WARPS + 2) * 32;
 constexpr int TMEM_COLS = 512;
-constexpr int BOX = 32 * 128;          // one warp's staged piece: 32 rows x 64 columns
+constexpr int BOX = 32 * 64;           // one warp's staged piece: 32 rows x 32 columns
 constexpr int A_BYTES = BM * BK * 2;
 
 // A tile is HALVES accumulators of BN columns side by side.
@@ -157,14 +158,14 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// 32 columns of one row, rounded, into a warp's staged piece (the 128-byte-swizzled layout of a tile
-// of 32 rows x 64 columns); `half`: which 32 of the 64.
+// 32 columns of one row, rounded, into a warp's staged piece (the 64-byte-swizzled layout of a tile of 32
+// rows x 32 columns: 16-byte chunks XORed with the row pair).
 template <typename T>
-__device__ __forceinline__ void stage_row(uint32_t piece, int lane, int half, const float (&v)[32]) {
+__device__ __forceinline__ void stage_row(uint32_t piece, int lane, const float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t chunk = (uint32_t)(half * 4 + j) ^ (uint32_t)(lane & 7);
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece + lane * 128 + chunk * 16),
+    const uint32_t chunk = (uint32_t)j ^ (uint32_t)((lane >> 1) & 3);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece + lane * 64 + chunk * 16),
                  "r"(pack2<T>(v[j * 8 + 0], v[j * 8 + 1])), "r"(pack2<T>(v[j * 8 + 2], v[j * 8 + 3])),
                  "r"(pack2<T>(v[j * 8 + 4], v[j * 8 + 5])), "r"(pack2<T>(v[j * 8 + 6], v[j * 8 + 7]))
                  : "memory");
@@ -176,23 +177,18 @@ __device__ __forceinline__ void store_elements(T* base, int64_t stride, uint32_t
                                                int M, int N) {
   const int rows = min(32, M - row0);
   for (int r = 0; r < rows; ++r) {
-    uint16_t* to = reinterpret_cast<uint16_t*>(base + (int64_t)(row0 + r) * stride + col0);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = h * 32 + lane;
-      const uint32_t chunk = (uint32_t)(c / 8) ^ (uint32_t)(r & 7);
-      uint16_t bits;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(piece + r * 128 + chunk * 16 + (c % 8) * 2) : "memory");
-      if (col0 + c < N) to[c] = bits;
-    }
+    const uint32_t chunk = (uint32_t)(lane / 8) ^ (uint32_t)((r >> 1) & 3);
+    uint16_t bits;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(piece + r * 64 + chunk * 16 + (lane % 8) * 2) : "memory");
+    if (col0 + lane < N) reinterpret_cast<uint16_t*>(base + (int64_t)(row0 + r) * stride + col0)[lane] = bits;
   }
 }
 
-// v += the next 64 of `left` elements; `packets`: they are 16-byte aligned.
+// v += the next 32 of `left` elements; `packets`: they are 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void add_row(float (&v)[2][32], const T* from, int left, bool packets) {
+__device__ __forceinline__ void add_row(float (&v)[32], const T* from, int left, bool packets) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     float e[8];
     if (packets && j * 8 + 8 <= left) {
       load_vec<T, 8>(from + j * 8, e);
@@ -201,7 +197,7 @@ __device__ __forceinline__ void add_row(float (&v)[2][32], const T* from, int le
       for (int i = 0; i < 8; ++i) e[i] = j * 8 + i < left ? to_f32(from[j * 8 + i]) : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[j / 4][(j % 4) * 8 + i] += e[i];
+    for (int i = 0; i < 8; ++i) v[j * 8 + i] += e[i];
   }
 }
 
@@ -383,7 +379,7 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue (warps 0-7)
+    // ------------------------------------------------------------ epilogue (warps 0-15)
     const int quarter = warp % 4, part = warp / 4;
     const uint32_t piece = smem_base + STAGES * STAGE_BYTES + warp * BOX;
     const Act act = (Act)a.act;
@@ -398,11 +394,10 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
       const int row0 = (tm * 2 + (int)rank) * BM + quarter * 32;
       const int row = row0 + lane;
       // out of a warp's registers into one of the outputs
-      auto emit = [&](const CUtensorMap* map, bool tma, void* base, int64_t stride, int col0, const float (&v)[2][32]) {
+      auto emit = [&](const CUtensorMap* map, bool tma, void* base, int64_t stride, int col0, const float (&v)[32]) {
         if (staged && lane == 0) tma_store_wait_read();
         __syncwarp();
-        stage_row<T>(piece, lane, 0, v[0]);
-        stage_row<T>(piece, lane, 1, v[1]);
+        stage_row<T>(piece, lane, v);
         if (tma) fence_proxy_async();
         __syncwarp();
         if (!tma) {
@@ -430,25 +425,21 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
           released = true;
         };
 #pragma unroll 1
-        for (int c = part * 64; c < COLS && row0 < a.M && first_col + c < a.N; c += 128) {
-          // one piece: 64 output columns
+        for (int c = part * 32; c < COLS && row0 < a.M && first_col + c < a.N; c += 128) {
+          // one piece: 32 output columns
           const int col0 = first_col + c;
           const bool last = c + 128 >= COLS || col0 + 128 >= a.N;
-          float v[2][32];
-          load_tmem(lanes + c, v[0]);
-          load_tmem(lanes + c + 32, v[1]);
+          float v[32];
+          load_tmem(lanes + c, v);
           if constexpr (GATED) {
-            float up[2][32];
-            load_tmem(lanes + BN / 2 + c, up[0]);
-            load_tmem(lanes + BN / 2 + c + 32, up[1]);
+            float up[32];
+            load_tmem(lanes + BN / 2 + c, up);
             if (last) release();
             if (a.pre) emit(&maps.pre, a.tma_pre, a.pre, a.spm, col0, v);
             if (a.pre2) emit(&maps.pre2, a.tma_pre, a.pre2, a.spm, col0, up);
             with_act(act, [&](auto tag) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[h][i] = act_forward<false>(decltype(tag)::value, v[h][i]) * up[h][i];
+              for (int i = 0; i < 32; ++i) v[i] = act_forward<false>(decltype(tag)::value, v[i]) * up[i];
             });
           } else {
             if (last) release();
@@ -457,9 +448,7 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
             if (act != Act::None)
               with_act(act, [&](auto tag) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) v[h][i] = act_forward<false>(decltype(tag)::value, v[h][i]);
+                for (int i = 0; i < 32; ++i) v[i] = act_forward<false>(decltype(tag)::value, v[i]);
               });
             if (a.residual && row < a.M)
               add_row<T>(v, (const T*)a.residual + (int64_t)row * a.srm + col0, a.N - col0, a.vec_residual);
@@ -487,8 +476,8 @@ std::string output_map(CUtensorMap* map, CUtensorMapDataType type, void* base, i
                        int64_t stride) {
   uint64_t dims[2] = {(uint64_t)N, (uint64_t)M};
   uint64_t strides[1] = {(uint64_t)(M > 1 ? stride : (N + 7) / 8 * 8) * 2};
-  uint32_t box[2] = {64u, 32u};
-  return make_tensor_map(map, type, 2, base, dims, strides, box);
+  uint32_t box[2] = {32u, 32u};
+  return make_tensor_map(map, type, 2, base, dims, strides, box, 64);
 }
 
 template <typename T, bool GATED, int BN, int HALVES>

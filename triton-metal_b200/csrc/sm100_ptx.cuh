@@ -444,11 +444,11 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }  // namespace ptx
 
 // ---- host: tensor maps ------------------------------------------------------------
-// 2-D / 3-D tiled tensor map with 128-byte swizzle.  dims/strides innermost first;
+// 2-D / 3-D tiled tensor map, swizzled over 128 bytes (or 64).  dims/strides innermost first;
 // strides (bytes) are given for dims 1.. (dim 0 is contiguous).  Returns an error
 // string or empty.
 std::string make_tensor_map(CUtensorMap* out, CUtensorMapDataType type, int rank, const void* base,
                             const uint64_t* dims, const uint64_t* strides_bytes,
-                            const uint32_t* box);
+                            const uint32_t* box, int swizzle_bytes = 128);
 
 }  // namespace tmc
