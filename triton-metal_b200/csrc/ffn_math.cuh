@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "ffn_core.h"
+#include "sm100_ptx.cuh"
 
 namespace tmc {
 namespace ffn {
@@ -64,6 +65,21 @@ constexpr float kInvSqrt2Pi = 0.39894228040143267794f;
 constexpr float kTanhA = 0.79788456080286535588f;   // sqrt(2 / pi)
 constexpr float kTanhB = 0.044715f;
 
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // The normal distribution's upper tail at |z|, 1 - Phi(|z|) = erfc(|z| / sqrt 2) / 2, for 16-bit results: the
 // rational approximation 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions (absolute error
 // below 1.5e-7 of erf), fourteen instructions without a branch where erff takes both of its two.  `density`
@@ -86,9 +102,10 @@ __device__ __forceinline__ float act_forward(Act act, float z) {
     case Act::Relu: return z != z ? z : fmaxf(z, 0.f);          // fmaxf alone would drop a NaN
     case Act::Gelu: {
       if constexpr (PRECISE) return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+      // z Phi(z) = max(z, 0) - |z| tail(|z|); |z| bounded where the tail is 0, so that infinities give the limits
       float density;
-      const float tail = normal_tail(z, density);
-      return z * (z < 0.f ? tail : 1.f - tail);
+      const float a = min_nan(fabsf(z), 100.f);
+      return max_nan(z, 0.f) - a * normal_tail(a, density);
     }
     case Act::GeluTanh: return z * sigmoid<PRECISE>(2.f * kTanhA * (z + kTanhB * z * z * z));
     case Act::Silu: return z * sigmoid<PRECISE>(z);
@@ -120,6 +137,38 @@ __device__ __forceinline__ float act_derivative(Act act, float z) {
       return s * (1.f - s);
     }
     default: return 1.f;
+  }
+}
+
+// The activation of a row's registers: gelu of 16-bit results two-wide (it is the dearest: with scalar
+// arithmetic 16384 x 1024 x 4096 ran at 1069 TFLOP/s, this way at 1169), the others element by element.
+template <Act ACT, int N>
+__device__ __forceinline__ void act_row(float (&v)[N]) {
+  if constexpr (ACT == Act::Gelu) {
+    auto both = [](float c) { return ptx::pack_f32x2(c, c); };
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float a0 = min_nan(fabsf(v[i]), 100.f), a1 = min_nan(fabsf(v[i + 1]), 100.f);
+      const uint64_t a = ptx::pack_f32x2(a0, a1);
+      // exp(-z^2 / 2) as a power of two
+      const uint64_t power = ptx::mul_f32x2(ptx::mul_f32x2(a, a), both(-0.5f * 1.44269504088896341f));
+      const uint64_t below = ptx::fma_f32x2(a, both(0.3275911f * 0.70710678118654752440f), both(1.f));
+      float p0, p1, b0, b1;
+      ptx::unpack_f32x2(power, p0, p1);
+      ptx::unpack_f32x2(below, b0, b1);
+      const uint64_t density = ptx::pack_f32x2(ptx::fast_exp2(p0), ptx::fast_exp2(p1));
+      const uint64_t t = ptx::pack_f32x2(fast_rcp(b0), fast_rcp(b1));
+      uint64_t poly = ptx::fma_f32x2(both(0.5f * 1.061405429f), t, both(-0.5f * 1.453152027f));
+      poly = ptx::fma_f32x2(poly, t, both(0.5f * 1.421413741f));
+      poly = ptx::fma_f32x2(poly, t, both(-0.5f * 0.284496736f));
+      poly = ptx::fma_f32x2(poly, t, both(0.5f * 0.254829592f));
+      const uint64_t tail = ptx::mul_f32x2(ptx::mul_f32x2(poly, t), density);
+      const uint64_t out = ptx::fma_f32x2(ptx::pack_f32x2(-a0, -a1), tail, ptx::pack_f32x2(max_nan(v[i], 0.f), max_nan(v[i + 1], 0.f)));
+      ptx::unpack_f32x2(out, v[i], v[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = act_forward<false>(ACT, v[i]);
   }
 }
 

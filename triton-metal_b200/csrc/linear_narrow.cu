@@ -12,8 +12,8 @@
 // the columns from all the shares through distributed shared memory, in rank order - no workspace, no
 // atomics, the same bits every time.
 //
-//   warp 4 TMA producer, warp 5 MMA issuer, warps 0-3 read TMEM (thread = output column); all six
-//   finish the cluster's sums.  About 100 KB of ring a CTA (two CTAs an SM) keep the memory bus busy:
+//   warps 0 ... 3 (7, 15 with more rows) read TMEM (thread = output column), then a TMA producer warp and an
+//   MMA issuer warp; all of them finish the cluster's sums.  About 100 KB of ring a CTA (two CTAs an SM) keep the memory bus busy:
 //   148 x 100 KB in flight against 6.5 TB/s x 1 us.
 
 #include "ffn_math.cuh"
@@ -30,10 +30,13 @@ using namespace ffn;
 
 constexpr int BN = 128;                // output columns of a CTA
 constexpr int BK = 64;
-constexpr int NUM_THREADS = 192;
 constexpr int W_BYTES = BN * BK * 2;
 
 template <int TOK, bool GATED> struct Config {
+  // the sums are finished by as many warps as there are rows to keep busy: what each does is short and waits
+  // for distributed shared memory, and unrolling it instead misses the instruction cache
+  static constexpr int EPI_WARPS = TOK <= 16 ? 4 : TOK <= 64 ? 8 : 16;
+  static constexpr int NUM_THREADS = (EPI_WARPS + 2) * 32;
   static constexpr int X_BYTES = TOK * BK * 2;
   static constexpr int STAGE_BYTES = W_BYTES * (GATED ? 2 : 1) + X_BYTES;
   // two CTAs an SM up to 64 rows, one beyond (the shares of a cluster must fit where the ring was)
@@ -93,6 +96,18 @@ __device__ __forceinline__ void add(float4& a, const float4& b) {
   a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
 }
 
+// The sum over the cluster of what lies at `addr` in each CTA's shared memory, in rank order.
+__device__ __forceinline__ float4 gather(uint32_t addr, int split) {
+  float4 part[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    if (r < split) part[r] = load_share(addr, r);
+#pragma unroll
+  for (int r = 1; r < 8; ++r)
+    if (r < split) add(part[0], part[r]);
+  return part[0];
+}
+
 // Four neighbouring elements of an output or a bias / residual: one 8-byte access where the address allows.
 template <typename T>
 __device__ __forceinline__ void add4(float (&v)[4], const T* from, int left, bool quads) {
@@ -123,7 +138,7 @@ __device__ __forceinline__ void put4(T* to, const float (&v)[4], int left, bool 
 }
 
 // Outputs n ... n + 3 of row m (`left` of them exist) from x w, and from x w2 of a gated product.
-template <typename T, bool GATED, Act ACT>
+template <typename T, bool GATED>
 __device__ __forceinline__ void finish(const Args& a, int64_t m, int n, int left, float4 sum, float4 sum2) {
   float z[4] = {sum.x, sum.y, sum.z, sum.w};
   if constexpr (GATED) {
@@ -131,22 +146,23 @@ __device__ __forceinline__ void finish(const Args& a, int64_t m, int n, int left
     if (a.pre) put4((T*)a.pre + m * a.spm + n, z, left, a.quads & kQuadPre);
     if (a.pre2) put4((T*)a.pre2 + m * a.spm + n, up, left, a.quads & kQuadPre);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>(ACT, z[i]) * up[i];
+    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>((Act)a.act, z[i]) * up[i];
   } else {
     if (a.bias) add4(z, (const T*)a.bias + n, left, a.quads & kQuadBias);
     if (a.pre) put4((T*)a.pre + m * a.spm + n, z, left, a.quads & kQuadPre);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>(ACT, z[i]);
+    for (int i = 0; i < 4; ++i) z[i] = act_forward<false>((Act)a.act, z[i]);
     if (a.residual) add4(z, (const T*)a.residual + m * a.srm + n, left, a.quads & kQuadResidual);
   }
   put4((T*)a.out + m * a.som + n, z, left, a.quads & kQuadOut);
 }
 
 template <typename T, int TOK, bool GATED>
-__global__ void __launch_bounds__(NUM_THREADS, TOK <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(Config<TOK, GATED>::NUM_THREADS, TOK <= 64 ? 2 : 1)
 linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a, DeviceStatus* status) {
   using C = Config<TOK, GATED>;
-  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES;
+  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES, NUM_THREADS = C::NUM_THREADS;
+  constexpr int PRODUCER = C::EPI_WARPS, ISSUER = C::EPI_WARPS + 1;
   constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -186,7 +202,7 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
   // The thread that makes the barriers fills the ring at once: the first weights are under way while the
   // TMEM is allocated and the other warps arrive.
   const int ahead = min(STAGES, kb1 - kb0);
-  if (warp == 4 && lane == 0) {
+  if (warp == PRODUCER && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&bars.full[s]), 1);
       mbar_init(smem_u32(&bars.empty[s]), 1);
@@ -196,7 +212,7 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     fence_barrier_init();
     for (int s = 0; s < ahead; ++s) fetch(kb0 + s, s);
   }
-  if (warp == 5) {
+  if (warp == ISSUER) {
     tmem_alloc(smem_u32(&bars.tmem_base), C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -207,7 +223,7 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
   const uint32_t tmem_base = bars.tmem_base;
 
   bool ok = true;
-  if (warp == 4) {
+  if (warp == PRODUCER) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int stage = ahead == STAGES ? 0 : ahead;
@@ -228,7 +244,7 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
         }
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == ISSUER) {
     // ------------------------------------------------------------ MMA issuer
     constexpr uint32_t n_field = TOK;
     const uint32_t idesc = make_idesc(FMT, BN, n_field, a.w_mn, 0);
@@ -254,74 +270,51 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     if (ok) mma_commit_elect(smem_u32(&bars.acc_full));
   } else {
     // ------------------------------------------------------------ accumulator, thread = output column
-    ok = mbar_wait(smem_u32(&bars.acc_full), 0, wc, kEpiAccFull);
+    // (after a wait that gave up the sums are whatever is there, and the launch is reported as failed)
+    mbar_wait(smem_u32(&bars.acc_full), 0, wc, kEpiAccFull);
     tc_fence_after();
-    const uint32_t lanes = tmem_base + ((uint32_t)(warp * 32) << 16);
-    float* share = reinterpret_cast<float*>(smem);       // [GATED][row][128 columns]: the ring is idle now
+    const int quarter = warp % 4;
+    const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    float* share = reinterpret_cast<float*>(smem) + quarter * 32 + lane;     // [GATED][row][128 columns]: the ring is idle now
 #pragma unroll 1
-    for (int t = 0; t < rows && __all_sync(0xffffffffu, ok); t += 16) {
-      uint32_t z[16], up[16];
-      tmem_ld_32x16(lanes + t, z);
-      if constexpr (GATED) tmem_ld_32x16(lanes + TOK + t, up);
+    for (int t = warp / 4 * 8; t < rows; t += C::EPI_WARPS / 4 * 8) {
+      uint32_t z[8], up[8];
+      tmem_ld_32x8(lanes + t, z);
+      if constexpr (GATED) tmem_ld_32x8(lanes + TOK + t, up);
       tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (t + i >= rows) break;
-        share[(t + i) * BN + warp * 32 + lane] = __uint_as_float(z[i]);
-        if constexpr (GATED) share[(TOK + t + i) * BN + warp * 32 + lane] = __uint_as_float(up[i]);
+      for (int i = 0; i < 8; ++i) {           // (rows past the last are zeros in a place of their own)
+        share[(t + i) * BN] = __uint_as_float(z[i]);
+        if constexpr (GATED) share[(TOK + t + i) * BN] = __uint_as_float(up[i]);
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
-  // Four columns of a row at a time, four such pieces a thread and turn: the shares of the whole cluster are
-  // loaded for all of them before the first is added, since each load takes hundreds of clocks.
+  // Four columns of a row at a time, the shares of the whole cluster loaded before the first is added.
   if (a.split > 1) cluster_sync();     // every share is written
   const int width = BN / a.split, shift = 31 - __clz(width / 4), items = rows << shift;
-  with_act((Act)a.act, [&](auto tag) {
 #pragma unroll 1
-    for (int base = threadIdx.x; base < items; base += 4 * NUM_THREADS) {
-      float4 z[4], up[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = min(base + q * NUM_THREADS, items - 1), t = i >> shift, c = (int)rank * width + (i - (t << shift)) * 4;
-        const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
-        if (a.split == 1) {
-          z[q] = *reinterpret_cast<const float4*>(smem + (t * BN + c) * 4);
-          if constexpr (GATED) up[q] = *reinterpret_cast<const float4*>(smem + ((TOK + t) * BN + c) * 4);
-        } else {
-          z[q] = load_share(at, 0);
-          if constexpr (GATED) up[q] = load_share(at + TOK * BN * 4, 0);
-        }
-      }
-      for (int r = 1; r < a.split; ++r) {
-        float4 other[4], other_up[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int i = min(base + q * NUM_THREADS, items - 1), t = i >> shift, c = (int)rank * width + (i - (t << shift)) * 4;
-          const uint32_t at = smem_base + (uint32_t)(t * BN + c) * 4;
-          other[q] = load_share(at, r);
-          if constexpr (GATED) other_up[q] = load_share(at + TOK * BN * 4, r);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          add(z[q], other[q]);
-          if constexpr (GATED) add(up[q], other_up[q]);
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = base + q * NUM_THREADS, t = i >> shift, c = (int)rank * width + (i - (t << shift)) * 4;
-        const int left = a.N - n0 - c;
-        if (i < items && left > 0) finish<T, GATED, decltype(tag)::value>(a, m0 + t, n0 + c, left, z[q], up[q]);
-      }
+  for (int i = threadIdx.x; i < items; i += NUM_THREADS) {
+    const int t = i >> shift, c = (int)rank * width + (i - (t << shift)) * 4;
+    const int left = a.N - n0 - c;
+    if (left <= 0) continue;
+    const uint32_t at = (uint32_t)(t * BN + c) * 4;
+    float4 z, up = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.split == 1) {
+      z = *reinterpret_cast<const float4*>(smem + at);
+      if constexpr (GATED) up = *reinterpret_cast<const float4*>(smem + at + TOK * BN * 4);
+    } else {
+      z = gather(smem_base + at, a.split);
+      if constexpr (GATED) up = gather(smem_base + at + TOK * BN * 4, a.split);
     }
-  });
+    finish<T, GATED>(a, m0 + t, n0 + c, left, z, up);
+  }
   if (a.split > 1) {
     __syncwarp();
     cluster_sync();                    // nobody still reads this CTA's share
@@ -359,7 +352,7 @@ std::string launch_tok(const LinearProblem& p, const OperandLayout& lx, const Op
   if (err != cudaSuccess) return cudaGetErrorString(err);
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)((p.N + BN - 1) / BN * split), (unsigned)((p.M + TOK - 1) / TOK));
-  config.blockDim = dim3(NUM_THREADS);
+  config.blockDim = dim3(C::NUM_THREADS);
   config.dynamicSmemBytes = C::SMEM;
   config.stream = ctx.stream;
   cudaLaunchAttribute cluster{};
@@ -397,22 +390,23 @@ bool plan_linear_narrow(const LinearProblem& p, const OperandLayout& lx, int sm_
   if ((p.M + plan->rows - 1) / plan->rows > 65535 || tiles > 0x0fffffff) return false;
   const int64_t blocks = (p.K + BK - 1) / BK * (p.mode == LinearMode::Sum ? 2 : 1);
   const int64_t slots = (int64_t)sm_count * (plan->rows <= 64 ? 2 : 1);
-  // the split whose last CTA is done first: waves of CTAs times k-blocks each, plus the exchange
+  // The split that is done first.  An SM takes in about 38 bytes a clock (86 CTAs streamed 180 MB in 30 us), and
+  // what comes from memory comes at 3400 (6.5 TB/s at 1.9 GHz); the cluster's exchange costs about 2000 clocks, the
+  // rows of the sums 600 for every 512 groups of four columns.  Clusters of eight with an SM to each CTA do not
+  // all fit their GPCs at once, and take twice as long.
   double best = 0;
   plan->split = 0;
-  const int per_block = (p.mode == LinearMode::Gated ? 2 : 1) * 16 + plan->rows / 8;      // KB of a k-block
-  for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
+  const int weights = p.mode == LinearMode::Gated ? 2 : 1;
+  const double per_block = (double)(weights * 16384 + plan->rows * 128);
+  const double memory = 2.0 * ((double)p.K * (double)p.N * (p.w2 ? 2 : 1) + (double)p.M * (double)p.K) / 3400.0;
+  for (int split = 1; split <= (plan->rows <= 64 ? 8 : 4) && split <= blocks; split *= 2) {
     const int64_t ctas = tiles * split;
-    const int64_t each = (blocks + split - 1) / split;
-    // An SM takes in about 36 bytes a clock (86 CTAs streamed 180 MB in 30 us), all of them together 3400
-    // (6.5 TB/s at 1.9 GHz).
-    const double alone = (double)std::min<int64_t>(ctas, sm_count) * 36.0;
-    const double rate = std::min(alone, 3400.0) / (double)std::min<int64_t>(ctas, slots);      // bytes a clock of a CTA
-    const int64_t waves = (ctas + slots - 1) / slots;
-    // its rows of the sums, 768 groups of four columns a turn
+    const double each = (double)((blocks + split - 1) / split);
+    const double waves = (double)((ctas + slots - 1) / slots);
+    const double share = ctas > slots ? waves * (double)slots / sm_count : std::max(1.0, (double)ctas / sm_count);
     const double rows = (double)std::min<int64_t>(plan->rows, p.M);
-    const double finish = (split > 1 ? 2000.0 : 0.0) + rows * (32.0 / split) / (4 * NUM_THREADS) * (split > 1 ? 1500.0 : 1000.0);
-    const double time = (double)waves * ((double)each * per_block * 1024.0 / rate + finish);
+    const double finish = (split > 1 ? 2000.0 : 0.0) + rows * (32.0 / split) / 512.0 * 600.0;
+    const double time = std::max(memory, share * each * per_block / 38.0) + waves * finish;
     if (!plan->split || time < best) {
       best = time;
       plan->split = split;

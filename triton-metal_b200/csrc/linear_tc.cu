@@ -437,19 +437,15 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
             if (last) release();
             if (a.pre) emit(&maps.pre, a.tma_pre, a.pre, a.spm, col0, v);
             if (a.pre2) emit(&maps.pre2, a.tma_pre, a.pre2, a.spm, col0, up);
-            with_act(act, [&](auto tag) {
+            with_act(act, [&](auto tag) { act_row<decltype(tag)::value>(v); });
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = act_forward<false>(decltype(tag)::value, v[i]) * up[i];
-            });
+            for (int i = 0; i < 32; ++i) v[i] *= up[i];
           } else {
             if (last) release();
             if (a.bias) add_row<T>(v, (const T*)a.bias + col0, a.N - col0, a.vec_bias);
             if (a.pre) emit(&maps.pre, a.tma_pre, a.pre, a.spm, col0, v);
             if (act != Act::None)
-              with_act(act, [&](auto tag) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = act_forward<false>(decltype(tag)::value, v[i]);
-              });
+              with_act(act, [&](auto tag) { act_row<decltype(tag)::value>(v); });
             if (a.residual && row < a.M)
               add_row<T>(v, (const T*)a.residual + (int64_t)row * a.srm + col0, a.N - col0, a.vec_residual);
           }
@@ -524,16 +520,16 @@ std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const O
 }
 
 // Clocks of a launch with tiles of 256 x `width` accumulator columns.  What an SM takes in bounds the narrower
-// ones: about 56 bytes a clock, against the 64 that a 256-column k-block's 512 clocks of products ask for (96 of
-// a 128-column one, 48 of a 512-column one).  The widest leaves no second accumulator, so half of its epilogue is
-// not hidden under the next tile's products.
+// ones: a k-block's products take 256, 512 and 1024 clocks at 128, 256 and 512 columns and ask for 96, 64 and 48
+// bytes a clock; measured on 8192 x 4096 x 16384, 281, 420 and 791 ns a k-block of every pair.  The widest leaves no
+// second accumulator, so part of its epilogue is not hidden under the next tile's products.
 double tile_clocks(const LinearProblem& p, int width, int sm_count) {
   const int64_t cols = p.mode == LinearMode::Gated ? width / 2 : width;
   const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + cols - 1) / cols) * (p.mode == LinearMode::Pair ? 2 : 1);
   const int64_t blocks = (p.K + BK - 1) / BK * (p.mode == LinearMode::Sum ? 2 : 1);
   const int64_t waves = (tiles + sm_count / 2 - 1) / (sm_count / 2);
   const bool light = p.act == Act::None && p.mode != LinearMode::Gated && !p.pre && !p.residual;
-  const double block = width == 512 ? 1040.0 : width == 256 ? 570.0 : 430.0;
+  const double block = width == 512 ? 1040.0 : width == 256 ? 552.0 : 380.0;
   return (double)waves * ((double)blocks * block + (width == 512 ? (light ? 2000.0 : 6000.0) : 300.0));
 }
 // The width that is done first.
@@ -576,11 +572,11 @@ std::string make_operand_map(CUtensorMap* map, CUtensorMapDataType type, const v
 }
 
 double estimate_linear_tc(const LinearProblem& p, int sm_count) {
-  // With few rows it is bound by its operands' way from memory, at 2600 bytes a clock (it keeps fewer of them
-  // in flight than the kernel for few rows: 235 MB of gated weights took 49 us here, 41 us there).
+  // Few tiles get less of it than many do (128 x 4096 x 4096: 516 clocks a 128-column k-block), and a launch takes
+  // 5 us with nothing to do.  With few rows it is bound by its operands' way from memory, at 2600 bytes a clock.
   const double bytes = 2.0 * ((double)p.K * (double)p.N * (p.w2 ? 2 : 1) + (double)p.M * (double)p.K);
-  const double products = tile_clocks(p, tile_width(p, sm_count), sm_count);
-  return std::max(products, bytes / 2600.0) + 14000.0;
+  const double products = 1.33 * tile_clocks(p, tile_width(p, sm_count), sm_count);
+  return std::max(products, bytes / 2600.0) + 9500.0;
 }
 
 std::string launch_linear_tc(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw,
