@@ -55,9 +55,9 @@ __device__ __forceinline__ uint4 load_unaligned(const uint16_t* from) {
 __global__ void __launch_bounds__(256) align_operands_kernel(const CopyJobs jobs) {
   const CopyJob& j = jobs.job[blockIdx.y];
   const int64_t packets = j.pitch / 8, total = j.rows * packets;
-#pragma unroll 2
+  const uint32_t narrow = total < 0x7fffffff ? (uint32_t)packets : 0;      // a 64-bit division costs a hundred instructions
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / packets, c = (i - r * packets) * 8;
+    const int64_t r = narrow ? (int64_t)((uint32_t)i / narrow) : i / packets, c = (i - r * packets) * 8;
     const uint16_t* from = j.from + r * j.row_stride + c * j.col_stride;
     uint4 v;
     // (a packet's first word may begin two bytes early: at the operand's own first element that is not ours)

@@ -348,7 +348,8 @@ std::string launch_tok(const LinearProblem& p, const OperandLayout& lx, const Op
   a.quads = quad(p.out, nullptr, p.som, kQuadOut) | quad(p.pre, p.pre2, p.spm, kQuadPre) | quad(p.bias, nullptr, 0, kQuadBias) |
             quad(p.residual, nullptr, p.srm, kQuadResidual);
   auto kernel = linear_narrow_kernel<T, TOK, GATED>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  static const cudaError_t sized = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  cudaError_t err = sized;
   if (err != cudaSuccess) return cudaGetErrorString(err);
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)((p.N + BN - 1) / BN * split), (unsigned)((p.M + TOK - 1) / TOK));

@@ -507,7 +507,8 @@ std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const O
   if (e.empty() && a.tma_pre && p.pre2) e = output_map(&maps.pre2, type, p.pre2, p.M, p.N, p.spm);
   if (!e.empty()) return e;
   auto kernel = linear_tc_kernel<T, GATED, BN, HALVES>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  static const cudaError_t sized = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  cudaError_t err = sized;
   if (err != cudaSuccess) return cudaGetErrorString(err);
   const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + HALVES * COLS - 1) / (HALVES * COLS)) * (p.mode == LinearMode::Pair ? 2 : 1);
   if (tiles > 0x3fffffff) return "too many tiles";

@@ -24,6 +24,7 @@
 #include "sm100_ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace tmc {
 namespace {
@@ -772,11 +773,21 @@ std::string launch_stream(const NormProblem& p, const LaunchCtx& ctx, bool backw
                         : (const void*)residual_norm_bwd_stream_kernel<T, THREADS, PACKS, true, false>)
                 : (full ? (const void*)residual_norm_bwd_stream_kernel<T, THREADS, PACKS, false, true>
                         : (const void*)residual_norm_bwd_stream_kernel<T, THREADS, PACKS, false, false>);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  int resident = 1;
-  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, THREADS, smem);
-  if (e != cudaSuccess) return cudaGetErrorString(e);
-  const int64_t grid = std::min<int64_t>(std::max<int64_t>(p.M, 1), (int64_t)ctx.sm_count * std::max(resident, 1));
+  // blocks of this kernel and ring an SM holds, asked for once: the kernel's number, the ring's size, the answer
+  static std::atomic<uint64_t> known[5];
+  const int which = !backward ? 0 : 1 + (branch ? 2 : 0) + (full ? 1 : 0);
+  cudaError_t e = cudaSuccess;
+  uint64_t entry = known[which].load(std::memory_order_relaxed);
+  if (entry >> 8 != smem) {
+    int blocks = 1;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, THREADS, smem);
+    if (e != cudaSuccess) return cudaGetErrorString(e);
+    entry = (uint64_t)smem << 8 | (uint64_t)std::max(blocks, 1);
+    known[which].store(entry, std::memory_order_relaxed);
+  }
+  const int resident = (int)(entry & 255);
+  const int64_t grid = std::min<int64_t>(std::max<int64_t>(p.M, 1), (int64_t)ctx.sm_count * resident);
   if (!backward) {
     residual_norm_stream_kernel<T, THREADS, PACKS><<<(unsigned)grid, THREADS, smem, ctx.stream>>>(p, stages, ctx.status);
     ++*ctx.launches;

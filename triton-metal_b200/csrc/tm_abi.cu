@@ -598,7 +598,8 @@ bool regions_overlap(const Region& a, const Region& b, int eb) {
 struct InPlace {
   const void *out, *in;
 };
-bool check_aliasing(const std::vector<Region>& outputs, const std::vector<Region>& inputs, int eb,
+template <typename List>
+bool check_aliasing(const List& outputs, const List& inputs, int eb,
                     std::initializer_list<InPlace> allowed, std::string& err) {
   for (size_t i = 0; i < outputs.size(); ++i) {
     const Region& o = outputs[i];
@@ -628,6 +629,43 @@ bool check_aliasing(const std::vector<Region>& outputs, const std::vector<Region
   return true;
 }
 
+// The arguments of a feed-forward launch by role.  (Arrays, filled straight from the call by
+// tmx_launch_on: the smallest of these kernels run for 3 us.)
+struct Operands {
+  static constexpr int kRoles = (int)Role::Last + 1;
+  void* ptr[kRoles];
+  int64_t length[kRoles];     // bytes; -1: not an argument
+  int64_t number[kRoles];
+  bool has_number[kRoles];
+  float scalar[kRoles];
+  Operands() {
+    std::memset(this, 0, sizeof(*this));
+    for (int64_t& n : length) n = -1;
+  }
+};
+Operands operands_of(const Decoded& d) {
+  Operands o;
+  for (auto& kv : d.buffers) {
+    o.ptr[kv.first] = kv.second->ptr;
+    o.length[kv.first] = kv.second->length;
+  }
+  for (auto& kv : d.ints) {
+    o.number[kv.first] = kv.second;
+    o.has_number[kv.first] = true;
+  }
+  for (auto& kv : d.floats) o.scalar[kv.first] = kv.second;
+  return o;
+}
+struct RegionList {
+  Region item[16];
+  int count = 0;
+  void push_back(const Region& r) { item[count++] = r; }
+  const Region* begin() const { return item; }
+  const Region* end() const { return item + count; }
+  size_t size() const { return (size_t)count; }
+  const Region& operator[](size_t i) const { return item[i]; }
+};
+
 // One feed-forward launch, checked: everything that can be refused is refused by plan_feed_forward,
 // which looks at no device.
 struct FeedForwardPlan {
@@ -637,34 +675,33 @@ struct FeedForwardPlan {
   NormProblem norm{};
 };
 
-bool plan_feed_forward(const KernelObj& k, const Decoded& d, int64_t gx, int64_t gy, FeedForwardPlan& plan,
+bool plan_feed_forward(const KernelObj& k, const Operands& o, int64_t gx, int64_t gy, FeedForwardPlan& plan,
                        std::string& err) {
   const KernelDesc& desc = k.desc;
   const int eb = elt_size(desc.elt);
-  auto buf = [&](Role r) -> const BufferObj* {
-    auto it = d.buffers.find((int)r);
-    return it == d.buffers.end() ? nullptr : it->second.get();
-  };
-  auto ptr = [&](Role r) -> void* { const BufferObj* b = buf(r); return b ? b->ptr : nullptr; };
+  auto has = [&](Role r) { return o.length[(int)r] >= 0; };
+  auto ptr = [&](Role r) { return o.ptr[(int)r]; };
   auto number = [&](Role r, int64_t fallback, const char* name, int64_t& to) {
-    to = get_int(d, r, fallback);
+    to = o.has_number[(int)r] ? o.number[(int)r] : fallback;
     if (to < 0) err = invalid_argument(std::string(name) + " must not be negative, got " + std::to_string(to));
     return to >= 0;
   };
-  auto f32 = [&](Role r) { auto it = d.floats.find((int)r); return it == d.floats.end() ? 0.f : it->second; };
+  auto f32 = [&](Role r) { return o.scalar[(int)r]; };
+  auto extent = [&](Role r, const char* name, int64_t rows, int64_t rs, int64_t cols, int64_t cs, int bytes) {
+    BufferObj view;                    // only its length is looked at
+    view.length = o.length[(int)r];
+    return check_extent(view, {{rows, rs}, {cols, cs}}, bytes, name, err);
+  };
   // Every operand as rows x cols; checked against its buffer, and recorded for the aliasing check.
-  std::vector<Region> inputs, outputs;
-  auto operand = [&](Role r, const char* name, int64_t rows, int64_t cols, int64_t rs, int64_t cs, bool output,
-                     int bytes = 0) {
-    const BufferObj* b = buf(r);
-    if (!b) return true;
-    bytes = bytes ? bytes : eb;
-    if (!check_extent(*b, {{rows, rs}, {cols, cs}}, bytes, name, err)) return false;
-    if ((uintptr_t)b->ptr % (size_t)bytes) {
+  RegionList inputs, outputs;
+  auto operand = [&](Role r, const char* name, int64_t rows, int64_t cols, int64_t rs, int64_t cs, bool output) {
+    if (!has(r)) return true;
+    if (!extent(r, name, rows, rs, cols, cs, eb)) return false;
+    if ((uintptr_t)ptr(r) % (size_t)eb) {
       err = invalid_argument(std::string(name) + " is not aligned to its element size");
       return false;
     }
-    (output ? outputs : inputs).push_back(Region{name, b->ptr, rows, cols, rs, cs});
+    (output ? outputs : inputs).push_back(Region{name, ptr(r), rows, cols, rs, cs});
     return true;
   };
   if (is_linear(desc.id)) {
@@ -715,7 +752,7 @@ bool plan_feed_forward(const KernelObj& k, const Decoded& d, int64_t gx, int64_t
     p.M = M; p.N = N;
     if (!check_int32(M, "M", err) || !check_int32(N, "N", err)) return false;
     if (N == 0) return true;
-    if (!p.gated && p.act != Act::None && !buf(Role::Pre)) {
+    if (!p.gated && p.act != Act::None && !has(Role::Pre)) {
       err = invalid_argument("activation_bwd_kernel needs the pre-activations for this activation");
       return false;
     }
@@ -753,12 +790,12 @@ bool plan_feed_forward(const KernelObj& k, const Decoded& d, int64_t gx, int64_t
       err = invalid_argument("eps must not be negative");
       return false;
     }
-    const bool branch = buf(Role::Gate) || buf(Role::PostWeight);
-    if (!buf(Role::Block) && branch) {
+    const bool branch = has(Role::Gate) || has(Role::PostWeight);
+    if (!has(Role::Block) && branch) {
       err = invalid_argument("a gate or a norm behind the block needs the block's output");
       return false;
     }
-    if (backward && ((buf(Role::DGate) && !buf(Role::Gate)) || (buf(Role::DPost) && !buf(Role::PostWeight)))) {
+    if (backward && ((has(Role::DGate) && !has(Role::Gate)) || (has(Role::DPost) && !has(Role::PostWeight)))) {
       err = invalid_argument("a gradient was asked for of a gate or post weight that is not there");
       return false;
     }
@@ -786,22 +823,23 @@ bool plan_feed_forward(const KernelObj& k, const Decoded& d, int64_t gx, int64_t
                          {p.dresidual, p.dsum}, {p.dresidual, p.dnormed}, {p.dblock, p.dsum}, {p.dblock, p.dnormed},
                          {p.dblock, p.block}}, err))
       return false;
-    if (const BufferObj* stats = buf(Role::Stats)) {
+    if (has(Role::Stats)) {
       // four fp32 words a row, in 16-byte accesses; compared with the others as elements of their size
-      if (!check_extent(*stats, {{M, 4}, {4, 1}}, 4, "stats", err)) return false;
-      if ((uintptr_t)stats->ptr % 16) {
+      if (!extent(Role::Stats, "stats", M, 4, 4, 1, 4)) return false;
+      void* stats = ptr(Role::Stats);
+      if ((uintptr_t)stats % 16) {
         err = invalid_argument("stats is not aligned to 16 bytes");
         return false;
       }
       const int64_t row = 16 / eb;
-      const Region region{"stats", stats->ptr, M, row, row, 1};
-      for (auto& list : {outputs, inputs})
-        for (const Region& r : list)
+      const Region region{"stats", stats, M, row, row, 1};
+      for (const RegionList* list : {&outputs, &inputs})
+        for (const Region& r : *list)
           if (regions_overlap(region, r, eb)) {
             err = invalid_argument(std::string("stats overlaps ") + r.name + " in memory");
             return false;
           }
-      p.stats = (float*)stats->ptr;
+      p.stats = (float*)stats;
     }
     const bool sums = p.dweight || p.dbias || p.dgate || p.dpost;
     if (M == 0 && !sums) return true;
@@ -865,7 +903,7 @@ bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
     return false;
   }
   FeedForwardPlan plan;
-  if (is_feed_forward(k.desc.id) && !plan_feed_forward(k, d, gx, gy, plan, err)) return false;
+  if (is_feed_forward(k.desc.id) && !plan_feed_forward(k, operands_of(d), gx, gy, plan, err)) return false;
   if (!bind_device(err)) return false;
   {
     const std::string& why = unusable_reason();
@@ -1551,15 +1589,41 @@ int32_t tmx_launch_on(int64_t kernel, void* stream, int64_t gx, int64_t gy, int6
   if (k->binary || !is_feed_forward(k->desc.id))
     return fail(invalid_argument("tmx_launch_on takes the feed-forward kernels; the others run on the library's own stream"));
   if (!lengths) return fail(invalid_argument("tmx_launch_on received no lengths"));
+  // Addresses and numbers of the kinds the kernel declares are taken as they come; anything else (buffer
+  // handles, or something to refuse) goes through the general decoding.
+  Operands o;
   Decoded d;
-  if (!decode_args(*k, kinds, values, argc, d, err, lengths)) return fail(err);
+  const auto& declared = k->desc.args;
+  bool plain = kinds && values && argc == (int)declared.size();
+  for (int i = 0; plain && i < argc; ++i) {
+    const ArgInfo& a = declared[i];
+    const int role = (int)a.role;
+    if (a.is_pointer && kinds[i] == 4) {
+      if (lengths[i] < 0 || (values[i] == 0 && lengths[i] > 0))
+        return fail(invalid_argument("argument " + std::to_string(i) + " has no valid address and length"));
+      o.ptr[role] = (void*)(uintptr_t)values[i];
+      o.length[role] = lengths[i];
+    } else if (!a.is_pointer && kinds[i] == 3 && (a.role != Role::Scale && a.role != Role::Eps)) {
+      o.number[role] = values[i];
+      o.has_number[role] = true;
+    } else if (!a.is_pointer && kinds[i] == 2 && (a.role == Role::Scale || a.role == Role::Eps)) {
+      const uint32_t bits = (uint32_t)values[i];
+      std::memcpy(&o.scalar[role], &bits, 4);
+    } else {
+      plain = false;
+    }
+  }
+  if (!plain) {
+    if (!decode_args(*k, kinds, values, argc, d, err, lengths)) return fail(err);
+    for (int i = 0; i < argc; ++i)
+      if (kinds[i] == 4 && (lengths[i] < 0 || (values[i] == 0 && lengths[i] > 0)))
+        return fail(invalid_argument("argument " + std::to_string(i) + " has no valid address and length"));
+    o = operands_of(d);
+  }
   if (gx <= 0 || gy <= 0 || gz <= 0) return fail(invalid_argument("threadgroup grid must be positive in every dimension"));
   if (threads <= 0 || threads > 1024) return fail(invalid_argument("threadsPerThreadgroup must be 1...1024"));
-  for (int i = 0; i < argc; ++i)
-    if (kinds[i] == 4 && (lengths[i] < 0 || (values[i] == 0 && lengths[i] > 0)))
-      return fail(invalid_argument("argument " + std::to_string(i) + " has no valid address and length"));
   FeedForwardPlan plan;
-  if (!plan_feed_forward(*k, d, gx, gy, plan, err)) return fail(err);
+  if (!plan_feed_forward(*k, o, gx, gy, plan, err)) return fail(err);
   if (!ensure_device(err)) return fail(err);
   // the caller's current device is left as it was
   struct Restore {
@@ -1571,9 +1635,11 @@ int32_t tmx_launch_on(int64_t kernel, void* stream, int64_t gx, int64_t gy, int6
     restore.device = current;
     cudaSetDevice(g_dev.ordinal);
   }
-  {
+  static std::atomic<bool> usable{false};       // the probe's answer does not change
+  if (!usable.load(std::memory_order_relaxed)) {
     const std::string& why = unusable_reason();
     if (!why.empty()) return fail(cuda_error(why));
+    usable.store(true, std::memory_order_relaxed);
   }
   for (int i = 0; i < argc; ++i) {
     if (kinds[i] == 0 && stream != (void*)g_dev.stream)

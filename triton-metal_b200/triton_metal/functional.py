@@ -167,9 +167,9 @@ class _Recipe:
         slots = list(tensors)
         for slot, shape in self.copies:
             slots[slot] = slots[slot].reshape(shape).contiguous()
-        device = self.device
+        device, new = self.device, tensors[0].new_empty
         for shape, dtype in self.allocs:
-            slots.append(torch.empty(shape, dtype=dtype, device=device))
+            slots.append(new(shape) if dtype is self.dtype else new(shape, dtype=dtype))
         stream = _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
         for handle, gx, gy, threads, kinds, used, scalars, pack, lengths, n in self.steps:
             if _launch_on(handle, stream, gx, gy, 1, threads, kinds,
