@@ -140,6 +140,42 @@ __device__ __forceinline__ float act_derivative(Act act, float z) {
   }
 }
 
+// Value and derivative together: what both need - the sigmoid, the tail - is computed once.
+template <bool PRECISE>
+__device__ __forceinline__ void act_both(Act act, float z, float& value, float& slope) {
+  const float zb = bounded(z);
+  switch (act) {
+    case Act::Gelu: {
+      if constexpr (PRECISE) break;
+      float density;
+      const float tail = normal_tail(zb, density);
+      value = max_nan(z, 0.f) - fabsf(zb) * tail;
+      slope = fmaf(zb * kInvSqrt2Pi, density, zb < 0.f ? tail : 1.f - tail);
+      return;
+    }
+    case Act::GeluTanh: {
+      const float s = sigmoid<PRECISE>(2.f * kTanhA * (zb + kTanhB * zb * zb * zb));
+      value = z * s;
+      slope = s + zb * s * (1.f - s) * 2.f * kTanhA * (1.f + 3.f * kTanhB * zb * zb);
+      return;
+    }
+    case Act::Silu: {
+      const float s = sigmoid<PRECISE>(zb);
+      value = z * s;
+      slope = s * (1.f + zb * (1.f - s));
+      return;
+    }
+    case Act::Sigmoid: {
+      value = sigmoid<PRECISE>(zb);
+      slope = value * (1.f - value);
+      return;
+    }
+    default: break;
+  }
+  value = act_forward<PRECISE>(act, z);
+  slope = act_derivative<PRECISE>(act, z);
+}
+
 // The activation of a row's registers: gelu of 16-bit results two-wide (it is the dearest: with scalar
 // arithmetic 16384 x 1024 x 4096 ran at 1069 TFLOP/s, this way at 1169), the others element by element.
 template <Act ACT, int N>
