@@ -113,7 +113,7 @@ struct Feed {
 
 struct Form {
   int x_k, w_k;                      // the operand is contiguous along k
-  int x_packets, w_packets;
+  int x_packets, w_packets, out_packets;
   int split;
 };
 
@@ -121,12 +121,18 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float load_share(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ float4 load_share(uint32_t addr, uint32_t rank) {
   uint32_t remote;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote)
+               : "memory");
   return v;
+}
+__device__ __forceinline__ void add(float4& a, const float4& b) {
+  a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
 }
 
 __device__ __forceinline__ float finish(const LinearProblem& p, int64_t m, int64_t n, float z) {
@@ -194,23 +200,34 @@ __device__ __forceinline__ void finish_tile(const LinearProblem& p, const Form& 
   float* out = (float*)(second ? p.out2 : p.out);
   if (f.split > 1) cluster_sync();
   else __syncthreads();
+  // four columns of a row at a time: a share of another block takes hundreds of clocks to come
 #pragma unroll 1
-  for (int i = threadIdx.x; i < rows * COLS; i += 256) {
-    const int r = (int)rank * rows + i / COLS, c = i % COLS;
+  for (int i = threadIdx.x; i < rows * (COLS / 4); i += 256) {
+    const int r = (int)rank * rows + i / (COLS / 4), c = i % (COLS / 4) * 4;
     const int64_t m = m0 + r, n = n0 + c;
     if (m >= p.M || n >= p.N) continue;
-    float z = 0.f, up = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f), sum2 = sum;
     if (f.split > 1) {
       const uint32_t at = base + (uint32_t)(r * TN + c) * 4;
       for (int q = 0; q < f.split; ++q) {
-        z += load_share(at, q);
-        if constexpr (GATED) up += load_share(at + COLS * 4, q);
+        add(sum, load_share(at, q));
+        if constexpr (GATED) add(sum2, load_share(at + COLS * 4, q));
       }
     } else {
-      z = smem[r * TN + c];
-      if constexpr (GATED) up = smem[r * TN + COLS + c];
+      sum = *reinterpret_cast<const float4*>(&smem[r * TN + c]);
+      if constexpr (GATED) sum2 = *reinterpret_cast<const float4*>(&smem[r * TN + COLS + c]);
     }
-    out[m * p.som + n] = GATED ? finish_gated(p, m, n, z, up) : finish(p, m, n, z);
+    float z[4] = {sum.x, sum.y, sum.z, sum.w};
+    const float up[4] = {sum2.x, sum2.y, sum2.z, sum2.w};
+    const int left = (int)min((int64_t)4, p.N - n);
+    float* to = out + m * p.som + n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= left) break;
+      z[j] = GATED ? finish_gated(p, m, n + j, z[j], up[j]) : finish(p, m, n + j, z[j]);
+      if (!f.out_packets) to[j] = z[j];
+    }
+    if (f.out_packets) *reinterpret_cast<float4*>(to) = make_float4(z[0], z[1], z[2], z[3]);
   }
   if (f.split > 1) {
     __syncwarp();
@@ -378,11 +395,11 @@ std::string launch_tile(const LinearProblem& p, const LaunchCtx& ctx) {
   auto packets = [](const void* a, const void* b, int64_t stride) {
     return (((uintptr_t)a | (uintptr_t)b) % 16 == 0 && stride % 4 == 0) ? 1 : 0;
   };
-  // (an extent of one has a stride that is never stepped: the other dimension is the contiguous one)
   f.x_k = p.sxk == 1;
   f.w_k = p.swn != 1;
   f.x_packets = packets(p.x, p.x2, p.sxk);
   f.w_packets = packets(p.w, p.w2, p.swk);
+  f.out_packets = packets(p.out, p.out2, p.som) && p.N % 4 == 0;
   const int cols = GATED ? TN / 2 : TN;
   const int64_t gx = (p.M + TM - 1) / TM, gy = (p.N + cols - 1) / cols;
   const int64_t gz = p.mode == LinearMode::Pair ? 2 : 1;
