@@ -61,6 +61,14 @@ struct NormProblem {
   void *dresidual, *dblock, *dweight, *dbias, *dgate, *dpost;
 };
 
+// While it lives, the calling thread may set the library up (allocate, create streams, wait for its own probe)
+// although a stream of the thread is being captured: none of that touches the captured stream.
+struct SetUpDuringCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  SetUpDuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~SetUpDuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // Memory that lives from one point of the launch's stream to another (stream-ordered pool of the
 // library's own): two calls on two streams, or two captured graphs, never share it.
 std::string scratch_alloc(const LaunchCtx& ctx, size_t bytes, void** out);

@@ -15,6 +15,7 @@ namespace tmc {
 namespace {
 
 constexpr double kCopyFrom = 4e6;
+constexpr int64_t kMostRows = 0x7fffffff - 512;       // tiles past the edge are counted in 32 bits
 
 // The TMA's view of an operand of `outer` rows, K columns; false if it has none.
 bool layout_of(const void* base, const void* base2, int64_t outer, int64_t K, int64_t s_outer, int64_t s_k,
@@ -114,6 +115,7 @@ std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path
   const bool w_fits = layout_of(p.w, p.w2, p.N, p.K, p.swn, p.swk, &lw);
   const char* why = p.elt == Elt::F32 ? "fp32 operands take the CUDA cores"
                     : p.K == 0 ? "K is 0"
+                    : p.M > kMostRows || p.N > kMostRows || p.K > kMostRows ? "an extent within 512 of 2^31"
                     : path_option == 1 ? "the CUDA cores were asked for"
                     : path_option == 0 && work < kCopyFrom && !(x_fits && w_fits) ? "small, and not aligned to 16 bytes"
                                                                                  : nullptr;
@@ -132,7 +134,11 @@ std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path
   if (!w_fits) cw.plan(p.w, p.w2, p.N, p.K, p.swn, p.swk);
   void* scratch = nullptr;
   std::string e = scratch_alloc(ctx, cx.bytes + cw.bytes, &scratch);
-  if (!e.empty()) return e;
+  if (!e.empty()) {
+    if (path_option == 2) return e;
+    *path_used = 1;                      // no room for the copies: slower, but it needs none
+    return launch_linear_simt(p, ctx);
+  }
   char* at = (char*)scratch;
   CopyJobs jobs{};
   int n = 0;

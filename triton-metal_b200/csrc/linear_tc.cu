@@ -492,7 +492,7 @@ std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const O
   a.out = p.out; a.out2 = p.out2; a.pre = p.pre; a.pre2 = p.pre2;
   a.srm = p.srm; a.som = p.som; a.spm = p.spm;
   a.group_m = 8;                     // row blocks (of 256) walked together: 4, 16 and 32 were 2 to 7 % slower
-  auto aligned = [&](const void* q, int64_t stride) { return (uintptr_t)q % 16 == 0 && (p.M <= 1 || stride % 8 == 0); };
+  auto aligned = [&](const void* q, int64_t stride) { return (uintptr_t)q % 16 == 0 && (p.M <= 1 || (stride % 8 == 0 && stride < (1ll << 38))); };
   a.tma_out = aligned(p.out, p.som) && aligned(p.out2, p.som);
   a.tma_pre = aligned(p.pre, p.spm) && aligned(p.pre2, p.spm);
   a.vec_bias = (uintptr_t)p.bias % 16 == 0;

@@ -211,6 +211,7 @@ bool ensure_device(std::string& err) {
     return g_dev.ok;
   }
   g_dev.tried = true;
+  SetUpDuringCapture relaxed;
   auto fail = [&](const std::string& m) {
     g_dev.why = cuda_error(m);
     err = g_dev.why;
@@ -290,6 +291,7 @@ const std::string& unusable_reason() {
     return g_dev.unusable;
   }
   int got = 0;
+  SetUpDuringCapture relaxed;
   std::string e = launch_probe(launch_ctx(), &got);
   if (!e.empty()) g_dev.unusable = "probe kernel failed: " + e;
   else if (got != 0x7a11) g_dev.unusable = "probe kernel stored the wrong value";
@@ -1396,8 +1398,6 @@ int64_t tm_load_kernel(int64_t library, const char* name) {
         if (std::string(force) == "simt") obj->path_option = 1;
         else if (std::string(force) == "tcgen05") obj->path_option = 2;
       }
-      // the device probe waits for the GPU, which a stream capture forbids: run it before one
-      if (is_feed_forward(k.id)) unusable_reason();
       return g_handles.insert(obj);
     }
   }
@@ -1654,6 +1654,7 @@ int32_t tmx_launch_on(int64_t kernel, void* stream, int64_t gx, int64_t gy, int6
       return fail(invalid_argument("argument " + std::to_string(i) + " is not memory of device " +
                                    std::to_string(g_dev.ordinal)));
   }
+  SetUpDuringCapture relaxed;           // a kernel's first launch loads it
   LaunchCtx ctx = launch_ctx();
   ctx.stream = (cudaStream_t)stream;
   if (stream == (void*)g_dev.stream) {
