@@ -52,13 +52,14 @@ template <int BN, int HALVES> struct Config {
   static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * BOX + 2048;
 };
 
-enum Site : uint32_t { kProdEmpty = 41, kMmaFull = 42, kMmaAccEmpty = 43, kEpiAccFull = 44, kDrain = 45 };
+enum Site : uint32_t { kProdEmpty = 41, kMmaFull = 42, kMmaAccEmpty = 43, kEpiAccFull = 44, kDrain = 45, kTmemReady = 46 };
 
 struct Barriers {
   alignas(8) uint64_t full[8];
   alignas(8) uint64_t empty[8];
   alignas(8) uint64_t acc_full[2];
   alignas(8) uint64_t acc_empty[2];
+  alignas(8) uint64_t tmem_ready;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -241,15 +242,16 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
       mbar_init(smem_u32(&bars.acc_full[i]), 1);
       mbar_init(smem_u32(&bars.acc_empty[i]), 2 * EPI_WARPS);
     }
+    mbar_init(smem_u32(&bars.tmem_ready), 2);
     bars.abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == EPI_WARPS + 1) tmem_alloc_pair(smem_u32(&bars.tmem_base), TMEM_COLS);
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync();                       // the peer's barriers exist and both TMEM allocations are made
-  tc_fence_after();
-  const uint32_t tmem_base = bars.tmem_base;
+  if (warp == EPI_WARPS && lane == 0) {
+    tma_prefetch_desc(&maps.x);
+    tma_prefetch_desc(&maps.w);
+  }
+  __syncwarp();
+  cluster_sync();                       // both CTAs' barriers exist: the loads begin while the TMEM is allocated
 
   if (warp == EPI_WARPS) {
     // ------------------------------------------------------------ TMA producer
@@ -316,7 +318,13 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
     }
   } else if (warp == EPI_WARPS + 1) {
     // ------------------------------------------------------------ MMA issuer (leader only)
-    if (rank == 0) {
+    tmem_alloc_pair(smem_u32(&bars.tmem_base), TMEM_COLS);
+    tc_fence_before();
+    if (lane == 0) arrive_at(map_to_cta(smem_u32(&bars.tmem_ready), 0));
+    __syncwarp();
+    if (rank == 0 && mbar_wait_warp(smem_u32(&bars.tmem_ready), 0, wc, kTmemReady)) {
+      tc_fence_after();
+      const uint32_t tmem_base = *(volatile uint32_t*)&bars.tmem_base;
       const uint32_t idesc = make_idesc(FMT, 2 * BM, BN, a.x_mn, a.w_mn);
       const SmemDesc a_base = make_desc_sw128(smem_base, a.x_mn ? 8192 : 0, 1024);
       const SmemDesc b_base = make_desc_sw128(smem_base + A_BYTES, a.w_mn ? 8192 : 0, 1024);
@@ -414,7 +422,8 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
         const uint32_t turn = HALVES == 2 ? local & 1 : (local >> 1) & 1;
         if (!mbar_wait(smem_u32(&bars.acc_full[acc]), turn, wc, kEpiAccFull)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
+        // (the allocation is ordered before the products that filled the accumulator)
+        const uint32_t lanes = *(volatile uint32_t*)&bars.tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
         const int first_col = (tn * HALVES + half) * COLS;
         // the accumulator may be overwritten: tell the leader, from both CTAs
         bool released = false;
@@ -454,7 +463,7 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
         if (!released) release();
       }
     }
-    if (lane == 0) tma_store_wait_all();
+    if (lane == 0) tma_store_wait_read();    // the staged pieces must outlive the stores' reads
   }
 
   tc_fence_before();
@@ -462,7 +471,7 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
   cluster_sync();                       // nobody still reads, writes or signals the other's memory
   if (warp == EPI_WARPS + 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    tmem_dealloc_pair(*(volatile uint32_t*)&bars.tmem_base, TMEM_COLS);
   }
 }
 
