@@ -167,29 +167,38 @@ std::string launch_typed(const ActBwdProblem& p, const LaunchCtx& ctx) {
 struct SumOutputs {
   void* out[kMaxColumnSums];
 };
-// 16 columns and 64 shares of the rows a block: the rows come from L2, eight in flight a thread, and a few
-// hundred of them are what the backward passes leave.
-constexpr int SUM_COLS = 16, SUM_ROWS = 64;
-template <typename T>
-__global__ void __launch_bounds__(SUM_COLS * SUM_ROWS) column_sums_kernel(const float* __restrict__ partial, int64_t parts,
-                                                                          int64_t N, const SumOutputs outs) {
-  __shared__ float joined[SUM_ROWS][SUM_COLS + 1];
-  const int tx = threadIdx.x % SUM_COLS, ty = threadIdx.x / SUM_COLS;
-  const int64_t n = (int64_t)blockIdx.x * SUM_COLS + tx;
+// COLS columns and ROWS shares of the partial rows a block: the rows come from L2, eight in flight a thread.
+template <typename T, int COLS, int ROWS>
+__global__ void __launch_bounds__(COLS * ROWS) column_sums_kernel(const float* __restrict__ partial, int64_t parts, int64_t N,
+                                                                  const SumOutputs outs) {
+  __shared__ float joined[ROWS][COLS + 1];
+  const int tx = threadIdx.x % COLS, ty = threadIdx.x / COLS;
+  const int64_t n = (int64_t)blockIdx.x * COLS + tx;
   const float* base = partial + (int64_t)blockIdx.y * parts * N;
   float total = 0.f;
   if (n < N) {
 #pragma unroll 8
-    for (int64_t r = ty; r < parts; r += SUM_ROWS) total += base[r * N + n];
+    for (int64_t r = ty; r < parts; r += ROWS) total += base[r * N + n];
   }
   joined[ty][tx] = total;
   __syncthreads();
 #pragma unroll
-  for (int step = SUM_ROWS / 2; step > 0; step /= 2) {
+  for (int step = ROWS / 2; step > 0; step /= 2) {
     if (ty < step) joined[ty][tx] += joined[ty + step][tx];
     __syncthreads();
   }
   if (ty == 0 && n < N) ((T*)outs.out[blockIdx.y])[n] = from_f32<T>(joined[0][tx]);
+}
+
+template <typename T>
+void launch_sums(const float* partial, int64_t parts, int64_t N, int sets, const SumOutputs& outs, const LaunchCtx& ctx) {
+  auto grid = [&](int cols) { return dim3((unsigned)((N + cols - 1) / cols), (unsigned)sets); };
+  // As many threads as the SMs hold at once, so few columns are split over more rows: 3 x 4096 columns of 296 rows
+  // took 17 us with 64 shares, 7 with 8; 2 x 1023 of 740 rows 17 us with 8, 8 with 64.
+  const int64_t columns = N * sets;
+  if (columns >= 8192) column_sums_kernel<T, 32, 8><<<grid(32), 256, 0, ctx.stream>>>(partial, parts, N, outs);
+  else if (columns >= 4096) column_sums_kernel<T, 32, 32><<<grid(32), 1024, 0, ctx.stream>>>(partial, parts, N, outs);
+  else column_sums_kernel<T, 16, 64><<<grid(16), 1024, 0, ctx.stream>>>(partial, parts, N, outs);
 }
 
 }  // namespace
@@ -198,11 +207,9 @@ void launch_column_sums(Elt elt, const float* partial, int64_t parts, int64_t N,
                         const LaunchCtx& ctx) {
   SumOutputs outs{};
   for (int i = 0; i < sets; ++i) outs.out[i] = out[i];
-  const dim3 grid((unsigned)((N + SUM_COLS - 1) / SUM_COLS), (unsigned)sets);
-  constexpr int THREADS = SUM_COLS * SUM_ROWS;
-  if (elt == Elt::F32) column_sums_kernel<float><<<grid, THREADS, 0, ctx.stream>>>(partial, parts, N, outs);
-  else if (elt == Elt::BF16) column_sums_kernel<__nv_bfloat16><<<grid, THREADS, 0, ctx.stream>>>(partial, parts, N, outs);
-  else column_sums_kernel<__half><<<grid, THREADS, 0, ctx.stream>>>(partial, parts, N, outs);
+  if (elt == Elt::F32) launch_sums<float>(partial, parts, N, sets, outs, ctx);
+  else if (elt == Elt::BF16) launch_sums<__nv_bfloat16>(partial, parts, N, sets, outs, ctx);
+  else launch_sums<__half>(partial, parts, N, sets, outs, ctx);
   ++*ctx.launches;
 }
 

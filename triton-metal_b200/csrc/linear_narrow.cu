@@ -77,9 +77,10 @@ __device__ __forceinline__ uint32_t cta_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// (not the .aligned forms: a warp whose lanes have taken different roles may still be diverged here)
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ float4 load_share(uint32_t addr, uint32_t rank) {
   uint32_t remote;
