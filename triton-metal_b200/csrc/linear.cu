@@ -3,8 +3,9 @@
 // The tensor-core kernels fetch their operands by TMA, which needs one contiguous dimension, a 16-byte
 // aligned base and a pitch that is a multiple of 16 bytes.  An operand that misses that (an odd width, a
 // slice at an odd column, no contiguous dimension) is first copied into aligned scratch memory: one read
-// and one write of it, against a product on the CUDA cores at a thirtieth of the tensor cores' rate.
-// Below kCopyFrom multiply-adds the two launches and the scratch cost more than the CUDA cores need.
+// and one write of it, against a product on the CUDA cores that reads element by element and waits for each
+// step of 16 k (1 x 129 x 129: 36 us there, 5 with the copy; 300 x 511 x 513: 196 and 10).  Up to two such
+// steps the second launch and the scratch cost the caller more than they save the GPU.
 
 #include "ffn_core.h"
 #include "linear_tc.h"
@@ -14,7 +15,7 @@
 namespace tmc {
 namespace {
 
-constexpr double kCopyFrom = 4e6;
+constexpr int64_t kCopyFromK = 33;
 constexpr int64_t kMostRows = 0x7fffffff - 512;       // tiles past the edge are counted in 32 bits
 
 // The TMA's view of an operand of `outer` rows, K columns; false if it has none.
@@ -109,7 +110,6 @@ std::string launch_tensor(const LinearProblem& p, const OperandLayout& lx, const
 std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path_option, int* path_used,
                           std::string* refused) {
   *path_used = 1;
-  const double work = (double)p.M * (double)p.N * (double)p.K;
   OperandLayout lx{}, lw{};
   const bool x_fits = layout_of(p.x, p.x2, p.M, p.K, p.sxm, p.sxk, &lx);
   const bool w_fits = layout_of(p.w, p.w2, p.N, p.K, p.swn, p.swk, &lw);
@@ -117,7 +117,7 @@ std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path
                     : p.K == 0 ? "K is 0"
                     : p.M > kMostRows || p.N > kMostRows || p.K > kMostRows ? "an extent within 512 of 2^31"
                     : path_option == 1 ? "the CUDA cores were asked for"
-                    : path_option == 0 && work < kCopyFrom && !(x_fits && w_fits) ? "small, and not aligned to 16 bytes"
+                    : path_option == 0 && p.K < kCopyFromK && !(x_fits && w_fits) ? "short, and not aligned to 16 bytes"
                                                                                  : nullptr;
   if (why) {
     if (path_option == 2) {

@@ -865,7 +865,8 @@ std::string launch_typed(const NormProblem& p, const LaunchCtx& ctx, bool backwa
     bases |= (uintptr_t)q;
   if (bases % 16 == 0 && p.stride % VEC == 0 && p.D % VEC == 0) {
     const int64_t packets = p.D / VEC;
-    // (two rows of the backward pass's four operands, or one of the forward's, have to fit)
+    // (two rows of the backward pass's four operands, or one of the forward's, have to fit; at 64 packets a warp
+    // to a row without the ring took 104 us forward and 325 back where this takes 110 and 160)
     if (packets > 32 && (size_t)p.D * sizeof(T) * (backward ? 8 : 2) <= kRingBytes) {
       // As few warps a row as hold it: the block-wide sums are what a row waits for (4096 bf16 columns
       // forward and back: 91 and 158 us with two packets a thread, 132 and 173 with one).
