@@ -421,7 +421,8 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
       for (int half = 0; half < HALVES; ++half) {
         const int acc = HALVES == 2 ? half : local & 1;
         const uint32_t turn = HALVES == 2 ? local & 1 : (local >> 1) & 1;
-        if (!mbar_wait(smem_u32(&bars.acc_full[acc]), turn, wc, kEpiAccFull)) { ok = false; break; }
+        // (the lanes leave together: one that gave up alone would be missed by the next warp-wide load)
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full[acc]), turn, wc, kEpiAccFull))) { ok = false; break; }
         tc_fence_after();
         // (the allocation is ordered before the products that filled the accumulator)
         const uint32_t lanes = *(volatile uint32_t*)&bars.tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
