@@ -293,6 +293,8 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
 
   tc_fence_before();
   __syncthreads();
+  // The columns go back before the first wait for the cluster: a CTA that held them while it waited for a peer,
+  // and a peer that waits for columns of another launch in the same state, would wait for each other.
   if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
