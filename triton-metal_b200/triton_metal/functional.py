@@ -87,8 +87,9 @@ class _Recipe:
         for name, t in tensors.items():
             if t is None:
                 continue
-            if t.dtype != self.dtype and not (name == "stats" and t.dtype == torch.float32):
-                raise TypeError(f"{name} is {t.dtype}, expected {torch.float32 if name == 'stats' else self.dtype}")
+            expected = torch.float32 if name == "stats" else self.dtype
+            if t.dtype != expected:
+                raise TypeError(f"{name} is {t.dtype}, expected {expected}")
             if t.device != self.device:
                 raise ValueError(f"{name} is on {t.device}, the other operands are on {self.device}")
         self.tensors = tensors
