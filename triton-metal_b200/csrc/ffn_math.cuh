@@ -101,7 +101,9 @@ __device__ __forceinline__ float act_forward(Act act, float z) {
   switch (act) {
     case Act::Relu: return z != z ? z : fmaxf(z, 0.f);          // fmaxf alone would drop a NaN
     case Act::Gelu: {
-      if constexpr (PRECISE) return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+      // erfc keeps the tail's relative accuracy where 1 + erf cancels (z = -5: four per cent off, z < -5.6: 0);
+      // z is bounded below where erfc is 0, so that minus infinity gives 0, the limit
+      if constexpr (PRECISE) return 0.5f * (z < -100.f ? -100.f : z) * erfcf(-z * kSqrtHalf);
       // z Phi(z) = max(z, 0) - |z| tail(|z|); |z| bounded where the tail is 0, so that infinities give the limits
       float density;
       const float a = min_nan(fabsf(z), 100.f);
@@ -119,7 +121,7 @@ __device__ __forceinline__ float act_derivative(Act act, float z) {
   switch (act) {
     case Act::Relu: return z != z ? z : (z > 0.f ? 1.f : 0.f);
     case Act::Gelu: {
-      if constexpr (PRECISE) return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expf(-0.5f * z * z);
+      if constexpr (PRECISE) return 0.5f * erfcf(-z * kSqrtHalf) + z * kInvSqrt2Pi * expf(-0.5f * z * z);
       float density;
       const float tail = normal_tail(z, density);
       return fmaf(z * kInvSqrt2Pi, density, z < 0.f ? tail : 1.f - tail);
