@@ -102,3 +102,31 @@ def test_gelu_derivative_keeps_its_accuracy_for_negative_f32(F):
     z64 = z.double()
     left, right = upper_tail(-z64), z64 * phi(z64)
     within(derivative(F, z, "gelu"), left + right, (z64 * z64 + 8) * 2.0 ** -23 * (left + right.abs()) + tiny(torch.float32))
+
+
+# gelu, 16 bits: the tail is within 2.2e-5 of itself; its exponential's argument, up to z^2 / 2, is rounded a few
+# times (z^2 2^-23), the approximate exponential and quotient add a few units of 2^-23 each; then one rounding.
+def fast_tail_relative(z):
+    return 2.2e-5 + (z * z + 16) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("kernel", ["pairs", "few rows", "cuda cores"])
+@pytest.mark.parametrize("element", ["f16", "bf16"])
+def test_gelu_of_16_bits_is_within_its_rounding_in_the_tail(F, element, kernel):
+    dtype = TYPES[element]
+    z = values(dtype, -12, 0, 6000)
+    z64 = z.double()
+    want = z64 * upper_tail(-z64)
+    slack = fast_tail_relative(z64) * want.abs()
+    within(forward(F, z, "gelu", kernel), want, slack + half(dtype) * (want.abs() + slack) + tiny(dtype))
+
+
+@pytest.mark.parametrize("element", ["f16", "bf16"])
+def test_gelu_derivative_of_16_bits_is_within_its_rounding_in_the_tail(F, element):
+    dtype = TYPES[element]
+    z = values(dtype, -12, 0, 6000)
+    z64 = z.double()
+    left, right = upper_tail(-z64), z64 * phi(z64)
+    slack = fast_tail_relative(z64) * (left + right.abs())
+    want = left + right
+    within(derivative(F, z, "gelu"), want, slack + half(dtype) * (want.abs() + slack) + tiny(dtype))
