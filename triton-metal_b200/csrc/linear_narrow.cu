@@ -271,8 +271,9 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     if (ok) mma_commit_elect(smem_u32(&bars.acc_full));
   } else {
     // ------------------------------------------------------------ accumulator, thread = output column
-    // (after a wait that gave up the sums are whatever is there, and the launch is reported as failed)
-    mbar_wait(smem_u32(&bars.acc_full), 0, wc, kEpiAccFull);
+    // (after a wait that gave up the sums are whatever is there, and the launch is reported as failed; by vote, so
+    // that the lanes come to the warp-wide loads together whichever of them saw the barrier or gave up first)
+    mbar_wait_warp(smem_u32(&bars.acc_full), 0, wc, kEpiAccFull);
     tc_fence_after();
     const int quarter = warp % 4;
     const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16);
