@@ -151,10 +151,14 @@ int32_t tmx_launch_timed(int64_t kernel, int64_t grid_x, int64_t grid_y, int64_t
  * graph: the kernels keep nothing between calls, and what scratch memory they need is allocated and
  * freed in stream order.  A buffer handle (kind 0) is ordered by the library's stream and accepted only
  * there (stream == tmx_stream_handle()).  The calling thread's current device stays as it was.
- * A bounded wait that gives up inside the kernel is reported by the next synchronising tm_* call. */
+ * A bounded wait that gives up inside the kernel is reported once, by whichever comes first: the next tmx_launch_on,
+ * which then launches nothing, tmx_check_status, or a synchronising tm_* call. */
 int32_t tmx_launch_on(int64_t kernel, void *stream, int64_t grid_x, int64_t grid_y, int64_t grid_z,
                       int64_t threads_per_threadgroup, const int32_t *kinds, const int64_t *values,
                       const int64_t *lengths, int32_t arg_count);
+/* -1 if a bounded wait gave up in a launch that has finished and has not been reported yet, else 0.  It waits for
+ * nothing: synchronise the stream first to have its launches covered. */
+int32_t tmx_check_status(void);
 /* Wait for everything enqueued on the library's stream; surfaces device-side
  * status words (bounded waits that gave up) as -1. */
 int32_t tmx_synchronize(void);

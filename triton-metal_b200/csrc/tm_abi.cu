@@ -313,6 +313,19 @@ void join_reads() {
   g_dev.read_back.clear();
 }
 
+// Reports the record that a kernel leaves when one of its bounded waits gives up, once.  (Pinned memory: no wait.)
+bool take_status(const char* whose, std::string& err) {
+  std::lock_guard<std::recursive_mutex> guard(g_dev.order_lock);
+  if (*(volatile unsigned int*)&g_dev.status->code == 0) return true;
+  DeviceStatus s = *g_dev.status;
+  std::memset(g_dev.status, 0, sizeof(DeviceStatus));
+  err = cuda_error("kernel execution failed: a bounded wait gave up inside the kernel (code " +
+                   std::to_string(s.code) + ", site " + std::to_string(s.where) + ", block " +
+                   std::to_string(s.block) + ", detail " + std::to_string(s.extra) +
+                   "); the results of " + whose + " are not valid");
+  return false;
+}
+
 bool sync_stream(std::string& err) {
   join_reads();
   cudaError_t e = cudaStreamSynchronize(g_dev.stream);
@@ -320,16 +333,7 @@ bool sync_stream(std::string& err) {
     err = cuda_error(std::string("kernel execution failed: ") + cudaGetErrorString(e));
     return false;
   }
-  if (g_dev.status->code != 0) {
-    DeviceStatus s = *g_dev.status;
-    std::memset(g_dev.status, 0, sizeof(DeviceStatus));
-    err = cuda_error("kernel execution failed: a bounded wait gave up inside the kernel (code " +
-                     std::to_string(s.code) + ", site " + std::to_string(s.where) + ", block " +
-                     std::to_string(s.block) + ", detail " + std::to_string(s.extra) +
-                     "); the results of this launch are not valid");
-    return false;
-  }
-  return true;
+  return take_status("this launch", err);
 }
 
 // ---------------------------------------------------------------------------
@@ -1654,6 +1658,8 @@ int32_t tmx_launch_on(int64_t kernel, void* stream, int64_t gx, int64_t gy, int6
       return fail(invalid_argument("argument " + std::to_string(i) + " is not memory of device " +
                                    std::to_string(g_dev.ordinal)));
   }
+  // nothing on this path ever waits, so what an earlier launch left is reported by the next one
+  if (!take_status("an earlier launch", err)) return fail(err);
   SetUpDuringCapture relaxed;           // a kernel's first launch loads it
   LaunchCtx ctx = launch_ctx();
   ctx.stream = (cudaStream_t)stream;
@@ -1674,6 +1680,17 @@ int32_t tmx_launch_on(int64_t kernel, void* stream, int64_t gx, int64_t gy, int6
       if (!kv.second->borrowed) raw.push_back(kv.second.get());
     note_launch(raw);
   }
+  return 0;
+}
+
+// Without a wait: has a launch that has finished given up?
+int32_t tmx_check_status(void) {
+  {
+    std::lock_guard<std::mutex> guard(g_dev.lock);
+    if (!g_dev.ok) return 0;               // nothing has run
+  }
+  std::string err;
+  if (!take_status("an earlier launch", err)) { store_error(err); return -1; }
   return 0;
 }
 

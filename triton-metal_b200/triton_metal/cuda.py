@@ -22,6 +22,7 @@ EXPORTS = {
     "tmx_launch_timed": (_I32, _LAUNCH + (_I32, _F32P)),
     # (the arrays as plain addresses: ctypes arrays or packed bytes)
     "tmx_launch_on": (_I32, (_I64, _PTR, _I64, _I64, _I64, _I64, _PTR, _PTR, _PTR, _I32)),
+    "tmx_check_status": (_I32, ()),
     "tmx_synchronize": (_I32, ()),
     "tmx_buffer_write_async": (_I32, (_I64, _I64, _PTR, _I64)),
     "tmx_buffer_read_async": (_I32, (_I64, _I64, _PTR, _I64)),
@@ -103,6 +104,11 @@ def launch_on(kernel, stream, grid, threads, kinds, values, lengths) -> None:
     """Enqueue a feed-forward kernel on a CUDA stream of the caller's.  `kinds`, `values` and
     `lengths` are ctypes arrays (i32, i64, i64); kind ARG_DEVICE_ADDRESS passes raw device memory."""
     _ok(_lib.tmx_launch_on(kernel, stream, grid[0], grid[1], 1, threads, kinds, values, lengths, len(kinds)))
+
+
+def check_status() -> None:
+    """Raise if a bounded wait gave up in a launch that has finished; waits for nothing."""
+    _ok(_lib.tmx_check_status())
 
 
 def synchronize() -> None:

@@ -42,6 +42,15 @@ def release():
     _KERNELS.clear()
 
 
+def check():
+    """Raise if a kernel among the work that has finished gave up a wait: its results are not valid.
+
+    The kernels' waits are bounded.  One that runs out is reported by the next call of this module, which then
+    launches nothing; a program whose last call it may have been, or that replays graphs, synchronises and asks
+    here."""
+    cuda.check_status()
+
+
 def _kernel(cls, dtype, operands=(), activation=None, norm=None):
     key = (cls, dtype, operands, activation, norm)
     kern = _KERNELS.get(key)
