@@ -57,3 +57,50 @@ def test_row_statistics_are_float32_whatever_the_operands_are(calls, dtype):
         with pytest.raises(TypeError, match="stats is torch.(bfloat16|float16|float64), expected torch.float32"):
             functional.residual_norm_backward(dn, None, s, zeros(M, 4, dtype=other), w)
     assert len(calls) == 1
+
+
+def operator_calls(x, w, g):
+    """Every function once, on 64 x 64 operands (w also as a vector's source)."""
+    stats = on_cuda(torch.zeros(64, 4))
+    return {
+        "linear": lambda: functional.linear(x, w, activation="silu"),
+        "linear_backward": lambda: functional.linear_backward(g, x, w),
+        "gated_linear": lambda: functional.gated_linear(x, w, w),
+        "gated_linear_backward": lambda: functional.gated_linear_backward(g, x, w, w, g, g),
+        "residual_norm": lambda: functional.residual_norm(x, g, w[0]),
+        "residual_norm_backward": lambda: functional.residual_norm_backward(g, None, x, stats, w[0]),
+    }
+
+
+@pytest.mark.parametrize("name", sorted(operator_calls(None, None, None)))
+@pytest.mark.parametrize("which", ["x", "w"])
+def test_an_operand_that_requires_grad_is_refused(calls, name, which):
+    """The functions record no graph: with grad mode on, the operand's gradient would be missing without a word."""
+    t = {k: zeros(64, 64, dtype=torch.float32) for k in "xwg"}
+    call = lambda: operator_calls(**t)[name]()  # noqa: E731
+    call()
+    made = len(calls)
+    t[which] = t[which].clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="requires grad, and these functions record no graph"):
+        call()
+    assert len(calls) == made
+    with torch.no_grad():
+        call()
+    with torch.inference_mode():
+        call()
+    assert len(calls) == 3 * made
+    t[which] = t[which].detach()
+    call()
+
+
+def test_a_forward_mode_tangent_is_refused(calls):
+    from torch.autograd import forward_ad
+    x, w = zeros(8, 16, dtype=torch.float32), zeros(16, 24, dtype=torch.float32)
+    functional.linear(x, w)
+    with forward_ad.dual_level():
+        functional.linear(x, w)
+        dual = forward_ad.make_dual(x, torch.ones(8, 16).as_subclass(OnCuda))
+        for grad_mode in (torch.no_grad, torch.enable_grad):
+            with grad_mode(), pytest.raises(RuntimeError, match="x carries a forward-mode tangent"):
+                functional.linear(dual, w)
+    assert len(calls) == 2

@@ -12,7 +12,8 @@ float32, float16 or bfloat16.
 x may have leading dimensions ([..., K]); weights are [K, N] with either dimension contiguous, so a
 weight stored [N, K] is passed as its transposed view.  Gradients are explicit functions: they take
 what the forward pass returned and return new tensors (a weight's gradient in the layout of the
-weight).  The reference has no counterpart.
+weight).  No graph is recorded, so an operand that requires grad is refused while grad mode is on (and one
+that carries a forward-mode tangent always).  The reference has no counterpart.
 
 Every call goes through a recipe: the checks of shapes, types and strides, the temporaries, and the
 launches with everything but the addresses.  Recipes depend on the operands' metadata alone and are
@@ -24,6 +25,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _core, cuda, kernels
 
@@ -91,7 +93,7 @@ class _Recipe:
             raise TypeError(f"{first_name} is {first.dtype}; float32, float16 and bfloat16 are supported")
         if not first.is_cuda or first.device.index != cuda.get_device():
             raise ValueError(f"{first_name} is on {first.device}; this process's device is cuda:{cuda.get_device()}")
-        self.dtype, self.device = first.dtype, first.device
+        self.dtype, self.device, self.index = first.dtype, first.device, first.device.index
         self.width = first.element_size()
         for name, t in tensors.items():
             if t is None:
@@ -101,6 +103,8 @@ class _Recipe:
                 raise TypeError(f"{name} is {t.dtype}, expected {expected}")
             if t.device != self.device:
                 raise ValueError(f"{name} is on {t.device}, the other operands are on {self.device}")
+            if t.requires_grad and _grad_enabled():
+                raise RuntimeError(f"{name} requires grad" + _NO_GRAPH)
         self.tensors = tensors
         self.slots = {name: i for i, name in enumerate(tensors)}
         self.copies, self.allocs, self.steps, self.results = [], [], [], []
@@ -164,10 +168,11 @@ class _Recipe:
         slots = [present[n].slot for n in kern.pointers]
         n = len(kern.names)
         lengths = [present[n_].span() * (4 if n_ == "stats" else self.width) for n_ in kern.pointers]
-        pack = struct.Struct(f"{n}q")
+        pack = struct.Struct(f"{len(slots)}q").pack
+        numbers = struct.pack(f"{len(scalars)}q", *scalars)
         grid = kern._grid(scalars[0], scalars[1])
-        self.steps.append((kern.handle, grid[0], grid[1], kern.threads, kern._kinds, slots, tuple(scalars), pack.pack,
-                           pack.pack(*lengths, *([0] * len(scalars))), n))
+        self.steps.append((kern.handle, grid[0], grid[1], kern.threads, kern._kinds, slots, pack, numbers,
+                           pack(*lengths) + bytes(len(numbers)), n))
 
     def product(self, x, w, out):
         self.launch(kernels.Linear, dict(x=x, w=w, out=out),
@@ -177,19 +182,28 @@ class _Recipe:
         slots = list(tensors)
         for slot, shape in self.copies:
             slots[slot] = slots[slot].reshape(shape).contiguous()
-        device, new = self.device, tensors[0].new_empty
+        new = tensors[0].new_empty
         for shape, dtype in self.allocs:
             slots.append(new(shape) if dtype is self.dtype else new(shape, dtype=dtype))
-        stream = _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
-        for handle, gx, gy, threads, kinds, used, scalars, pack, lengths, n in self.steps:
-            if _launch_on(handle, stream, gx, gy, 1, threads, kinds,
-                          pack(*[slots[i].data_ptr() for i in used], *scalars), lengths, n):
+        stream = _raw_stream(self.index) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream
+        for handle, gx, gy, threads, kinds, used, pack, numbers, lengths, n in self.steps:
+            if _launch_on(handle, stream, gx, gy, 1, threads, kinds, pack(*[slots[i].data_ptr() for i in used]) + numbers,
+                          lengths, n):
                 raise RuntimeError(_core.last_error())
         results = [None if r is None else slots[r[0]] if r[1] is None else r[1](slots[r[0]]) for r in self.results]
         return results[0] if len(results) == 1 else tuple(results)
 
 
 _launch_on = cuda._lib.tmx_launch_on
+_grad_enabled = torch.is_grad_enabled
+_NO_GRAPH = (", and these functions record no graph: call them under torch.no_grad() (or on detached tensors) and take "
+             "the gradients from the backward functions")
+
+
+def _refuse_tangents(names, tensors):
+    for name, t in zip(names, tensors):
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} carries a forward-mode tangent" + _NO_GRAPH)
 
 
 def _keep(key, recipe):
@@ -202,8 +216,12 @@ def _keep(key, recipe):
 
 def _call(build, static, names, tensors):
     """Run the recipe for these operands, made by `build` on first sight of their metadata."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(names, tensors)
     try:
-        key = (build, static, tuple([None if t is None else (t.dtype, t.device, t.shape, t.stride()) for t in tensors]))
+        key = (build, static, _grad_enabled(),
+               tuple([None if t is None else (t.dtype, t.get_device(), t.shape, t.stride(), t.requires_grad)
+                      for t in tensors]))
         recipe = _RECIPES.get(key)
     except AttributeError:          # not a tensor: the recipe says which
         key = recipe = None
@@ -244,8 +262,9 @@ def _plan_linear(r, activation, pre):
 def linear(x, weight, bias=None, residual=None, activation="none", *, pre=False, out=None):
     """act(x @ weight + bias) + residual; with pre=True also x @ weight + bias, which the backward
     pass of an activation reads.  `out` may be `residual` itself."""
-    return _call(_plan_linear, (activation, bool(pre)), ("x", "weight", "bias", "residual", "out"),
-                 (x, weight, bias, residual, out))
+    result = _call(_plan_linear, (activation, bool(pre)), ("x", "weight", "bias", "residual", "out"),
+                   (x, weight, bias, residual, out))
+    return result
 
 
 def _weight_gradient(r, x, dz, weight):
