@@ -104,3 +104,18 @@ def test_a_forward_mode_tangent_is_refused(calls):
             with grad_mode(), pytest.raises(RuntimeError, match="x carries a forward-mode tangent"):
                 functional.linear(dual, w)
     assert len(calls) == 2
+
+
+def test_an_output_given_by_the_caller_counts_as_written(calls):
+    """A graph that saved the tensor for its backward pass has to notice."""
+    x, w, out = zeros(8, 16, dtype=torch.float32), zeros(16, 24, dtype=torch.float32), torch.ones(8, 24)
+    leaf = torch.ones(8, 24, requires_grad=True)
+    product = leaf * out                                   # saves out
+    before = out._version
+    with torch.no_grad():
+        assert functional.linear(x, w, out=on_cuda(out)) is not None
+    assert out._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        functional.linear(x, w, out=on_cuda(torch.ones(8, 24)))     # (such tensors have no version)

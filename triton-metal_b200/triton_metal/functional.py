@@ -26,6 +26,7 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _core, cuda, kernels
 
@@ -264,6 +265,8 @@ def linear(x, weight, bias=None, residual=None, activation="none", *, pre=False,
     pass of an activation reads.  `out` may be `residual` itself."""
     result = _call(_plan_linear, (activation, bool(pre)), ("x", "weight", "bias", "residual", "out"),
                    (x, weight, bias, residual, out))
+    if out is not None and not out.is_inference():
+        increment_version(out)          # a graph that saved it notices
     return result
 
 
