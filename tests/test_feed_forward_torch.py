@@ -119,3 +119,14 @@ def test_an_output_given_by_the_caller_counts_as_written(calls):
         product.sum().backward()
     with torch.inference_mode():
         functional.linear(x, w, out=on_cuda(torch.ones(8, 24)))     # (such tensors have no version)
+
+
+def test_a_view_that_negates_its_memory_is_refused(calls):
+    pair = torch.randn(16, 24, dtype=torch.complex64)
+    x, w = zeros(8, 16, dtype=torch.float32), on_cuda(pair.conj().imag)
+    assert w.is_neg()
+    functional.linear(x, on_cuda(pair.imag))               # the same metadata otherwise
+    with pytest.raises(ValueError, match="weight is a view that negates its memory"):
+        functional.linear(x, w)
+    functional.linear(x, on_cuda(pair.conj().imag.resolve_neg()))
+    assert len(calls) == 2

@@ -106,6 +106,8 @@ class _Recipe:
                 raise ValueError(f"{name} is on {t.device}, the other operands are on {self.device}")
             if t.requires_grad and _grad_enabled():
                 raise RuntimeError(f"{name} requires grad" + _NO_GRAPH)
+            if t.is_neg():
+                raise ValueError(f"{name} is a view that negates its memory; pass {name}.resolve_neg()")
         self.tensors = tensors
         self.slots = {name: i for i, name in enumerate(tensors)}
         self.copies, self.allocs, self.steps, self.results = [], [], [], []
@@ -221,7 +223,7 @@ def _call(build, static, names, tensors):
         _refuse_tangents(names, tensors)
     try:
         key = (build, static, _grad_enabled(),
-               tuple([None if t is None else (t.dtype, t.get_device(), t.shape, t.stride(), t.requires_grad)
+               tuple([None if t is None else (t.dtype, t.get_device(), t.shape, t.stride(), t.requires_grad, t.is_neg())
                       for t in tensors]))
         recipe = _RECIPES.get(key)
     except AttributeError:          # not a tensor: the recipe says which
