@@ -130,3 +130,17 @@ def test_a_view_that_negates_its_memory_is_refused(calls):
         functional.linear(x, w)
     functional.linear(x, on_cuda(pair.conj().imag.resolve_neg()))
     assert len(calls) == 2
+
+
+@pytest.mark.parametrize("gate_rows", [True, False])
+@pytest.mark.parametrize("up_rows", [True, False])
+def test_gated_gradients_keep_the_layout_of_their_own_weight(calls, gate_rows, up_rows):
+    M, K, N = 24, 40, 56
+    weights = [zeros(K, N) if rows else zeros(N, K).t() for rows in (gate_rows, up_rows)]
+    x, m = zeros(M, K), [zeros(M, N) for _ in range(3)]
+    dx, *grads = functional.gated_linear_backward(m[0], x, *weights, m[1], m[2])
+    assert dx.shape == x.shape
+    for grad, weight in zip(grads, weights):
+        assert grad.shape == weight.shape and grad.stride() == weight.stride()
+    products = [c["name"] for c in calls[2:]]
+    assert products == (["linear_pair_kernel"] if gate_rows == up_rows else ["linear_kernel"] * 2)

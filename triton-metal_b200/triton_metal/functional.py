@@ -352,7 +352,7 @@ def _plan_gated_linear_backward(r, activation):
     _activation(activation)
     r.shape("x", tuple(r.tensors["dh"].shape[:-1]) + tuple(r.tensors["x"].shape[-1:]))
     x = r.rows("x")
-    original = r.matrix("w_gate", x.cols)
+    originals = r.matrix("w_gate", x.cols), r.matrix("w_up", x.cols)
     wg, wu = _gated_weights(r, x.cols)
     r.shape("dh", tuple(r.tensors["x"].shape[:-1]) + (wg.cols,))
     for name in ("pre_gate", "pre_up"):
@@ -368,10 +368,14 @@ def _plan_gated_linear_backward(r, activation):
     a, b = wg.T, wu.T
     r.launch(kernels.LinearSum, dict(x=dg, w=a, x2=du, w2=b, out=dx),
              (M, K, N, dg.s0, dg.s1, a.s0, a.s1, dx.s0))
-    dwg, (a, b), first = _weight_gradient(r, x, dg, original)
-    dwu, (a2, b2), second = _weight_gradient(r, x, du, original)
-    r.launch(kernels.LinearPair, dict(x=a, w=b, x2=a2, w2=b2, out=dwg, out2=dwu),
-             (a.rows, b.cols, a.cols, a.s0, a.s1, b.s0, b.s1, dwg.s0))
+    dwg, (a, b), first = _weight_gradient(r, x, dg, originals[0])
+    dwu, (a2, b2), second = _weight_gradient(r, x, du, originals[1])
+    if first[1] is second[1]:
+        r.launch(kernels.LinearPair, dict(x=a, w=b, x2=a2, w2=b2, out=dwg, out2=dwu),
+                 (a.rows, b.cols, a.cols, a.s0, a.s1, b.s0, b.s1, dwg.s0))
+    else:                               # two layouts: two products
+        r.product(a, b, dwg)
+        r.product(a2, b2, dwu)
     r.results = [(dx.slot, None), first, second]
 
 
