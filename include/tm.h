@@ -294,6 +294,12 @@ int32_t tmx_selftest_bounded_wait(int64_t budget_cycles, int32_t *results);
 int64_t tmx_debug_attention_schedule(int32_t kind, int32_t bh, int32_t rows, int32_t n_ctx, int32_t causal,
                                      int32_t ctas, int32_t *items_out, int64_t capacity, int32_t *begin_out,
                                      int64_t *load_out);
+/* Which kernel a 16-bit product of the feed-forward section takes on a device with sm_count SMs, for inspection and
+ * tests.  mode: 0 linear, 1 gated, 2 sum, 3 pair; pre, residual: whether there is one; x_by_k: x is contiguous along
+ * K.  out[0...3]: 1 few-row kernel / 0 CTA pairs; rows of x a tile / accumulator columns a tile; the split of K;
+ * tiles (CTA pairs only).  0 / -1. */
+int32_t tmx_debug_linear_choice(int32_t mode, int32_t activation, int32_t pre, int32_t residual, int64_t M, int64_t N,
+                                int64_t K, int32_t x_by_k, int32_t sm_count, int64_t *out);
 /* Set the device status word from the host, as a kernel whose wait gave up would. */
 int32_t tmx_debug_inject_status(int32_t code, int32_t where, int32_t block, int32_t extra);
 

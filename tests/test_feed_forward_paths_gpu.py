@@ -6,6 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from ffn_shapes import FEW_ROWS, PAIRS  # noqa: E402
 from test_feed_forward_gpu import (F, TYPES, act64, check, dact64, half, normal, own_error, product_slack,  # noqa: E402,F401
                                    weight, SLOPE)
 
@@ -40,3 +41,79 @@ def test_gated_weights_in_two_layouts(F, element, layouts):
         for t, w, (want, slack) in zip(got, (x, wg, wu), gated_backward64(dh, x, wg, wu, g, u, "silu")):
             check(t, want, slack)
             assert t.stride() == w.stride()
+
+
+# ---- every kernel and tile of the 16-bit products -----------------------------------------------------------
+# (test_feed_forward_choice.py holds the shapes to what they are here for.)
+
+def products(kind, x, w, x2, w2, out_shape):
+    """LinearSum or LinearPair through the C entry, on any two strides of either operand."""
+    from triton_metal import kernels
+    element = {torch.bfloat16: "bf16", torch.float16: "f16"}[x.dtype]
+    kern = getattr(kernels, kind)(element)
+    outs = [torch.full(out_shape, 7.0, device="cuda", dtype=x.dtype) for _ in range(1 if kind == "LinearSum" else 2)]
+    try:
+        tensors = [x, w, x2, w2] + outs
+        M, K = x.shape
+        kern.launch_tensors(torch.cuda.current_stream().cuda_stream, [t.data_ptr() for t in tensors],
+                            [t.numel() * t.element_size() for t in tensors],
+                            (M, w.shape[1], K, *x.stride(), *w.stride(), outs[0].stride(0)))
+        torch.cuda.synchronize()
+    finally:
+        kern.release()
+    return outs
+
+
+def product64(x, w):
+    x, w = x.double(), w.double()
+    return x @ w, (x.shape[1] + 2) * 2.0 ** -23 * (x.abs() @ w.abs())
+
+
+def check_case(F, mode, M, N, K, epilogue, dtype, layout):
+    if mode == "linear":
+        x, w = normal(M, K, dtype=dtype), weight(K, N, dtype, layout)
+        z, slack = product64(x, w)
+        if not epilogue:
+            return check(F.linear(x, w), z, slack)
+        bias, r = normal(N, dtype=dtype, std=0.3), normal(M, N, dtype=dtype)
+        out, pre = F.linear(x, w, bias, r, activation="gelu", pre=True)
+        z = z + bias.double()
+        slack = slack + 2.0 ** -23 * (z.abs() + bias.double().abs())
+        check(pre, z, slack, "pre")
+        want = act64(z, "gelu") + r.double()
+        return check(out, want, SLOPE * slack + own_error(z, dtype) + 2.0 ** -23 * want.abs(), "out")
+    if mode == "gated":
+        x, wg, wu = normal(M, K, dtype=dtype), weight(K, N, dtype, layout), weight(K, N, dtype, layout)
+        (g, eg), (u, eu) = product64(x, wg), product64(x, wu)
+        got = F.gated_linear(x, wg, wu, activation="gelu" if epilogue else "silu", save=bool(epilogue))
+        name = "gelu" if epilogue else "silu"
+        if epilogue:
+            check(got[1], g, eg, "gate")
+            check(got[2], u, eu, "up")
+            got = got[0]
+        a, ea = act64(g, name), SLOPE * eg + own_error(g, dtype)
+        return check(got, a * u, ea * (u.abs() + eu) + a.abs() * eu + 2.0 ** -23 * (a * u).abs(), "h")
+    if mode == "sum":
+        x, x2 = normal(M, K, dtype=dtype), normal(M, K, dtype=dtype)
+        w, w2 = weight(K, N, dtype, layout), weight(K, N, dtype, layout)
+        (a, ea), (b, eb) = product64(x, w), product64(x2, w2)
+        both = (K + 2) * 2.0 ** -23 * (x.double().abs() @ w.double().abs() + x2.double().abs() @ w2.double().abs())
+        return check(products("LinearSum", x, w, x2, w2, (M, N))[0], a + b, ea + eb + both)
+    x, x2 = normal(K, M, dtype=dtype).t(), normal(K, M, dtype=dtype).t()        # x^T dz: contiguous along m
+    w, w2 = (weight(K, N, dtype, layout) for _ in range(2))
+    for got, (want, slack) in zip(products("LinearPair", x, w, x2, w2, (M, N)), (product64(x, w), product64(x2, w2))):
+        check(got, want, slack)
+
+
+@pytest.mark.parametrize("case", PAIRS, ids=str)
+@pytest.mark.parametrize("element,layout", [("bf16", "kn"), ("f16", "nk")])
+def test_tiles_of_the_cta_pairs(F, case, element, layout):
+    mode, M, N, K, epilogue = case[:5]
+    check_case(F, mode, M, N, K, epilogue, TYPES[element], layout)
+
+
+@pytest.mark.parametrize("case", FEW_ROWS, ids=str)
+@pytest.mark.parametrize("element,layout", [("bf16", "nk"), ("f16", "kn")])
+def test_tiles_of_the_few_row_kernel(F, case, element, layout):
+    mode, M, N, K = case[:4]
+    check_case(F, mode, M, N, K, "pre" if mode != "sum" and M % 2 else "", TYPES[element], layout)

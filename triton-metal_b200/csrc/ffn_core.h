@@ -88,6 +88,13 @@ std::string launch_linear_f32(const LinearProblem& p, const LaunchCtx& ctx);
 // not) and reports which it was (1 or 2).
 std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path_option, int* path_used,
                           std::string* refused);
+// What a 16-bit product on the tensor cores runs on: the few-row kernel (tile: rows of x, split: of K) or the CTA
+// pairs (tile: accumulator columns, tiles: how many).
+struct TensorChoice {
+  int narrow, tile, split;
+  int64_t tiles;
+};
+TensorChoice tensor_choice(const LinearProblem& p, bool x_by_k, int sm_count);
 std::string launch_activation_bwd(const ActBwdProblem& p, const LaunchCtx& ctx);
 std::string launch_residual_norm(const NormProblem& p, const LaunchCtx& ctx);
 std::string launch_residual_norm_bwd(const NormProblem& p, const LaunchCtx& ctx);

@@ -98,14 +98,30 @@ struct Aligned {
 };
 
 // The kernel for few rows or the one for many, whichever its estimate says is done first.
+bool takes_narrow(const LinearProblem& p, const OperandLayout& lx, int sm_count, NarrowPlan* plan) {
+  return plan_linear_narrow(p, lx, sm_count, plan) && plan->clocks < estimate_linear_tc(p, sm_count);
+}
 std::string launch_tensor(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw, const LaunchCtx& ctx) {
   NarrowPlan narrow{};
-  if (plan_linear_narrow(p, lx, ctx.sm_count, &narrow) && narrow.clocks < estimate_linear_tc(p, ctx.sm_count))
-    return launch_linear_narrow(p, lx, lw, narrow, ctx);
+  if (takes_narrow(p, lx, ctx.sm_count, &narrow)) return launch_linear_narrow(p, lx, lw, narrow, ctx);
   return launch_linear_tc(p, lx, lw, ctx);
 }
 
 }  // namespace
+
+TensorChoice tensor_choice(const LinearProblem& p, bool x_by_k, int sm_count) {
+  NarrowPlan narrow{};
+  TensorChoice c{};
+  if (takes_narrow(p, OperandLayout{x_by_k ? 0 : 1, 0}, sm_count, &narrow)) {
+    c.narrow = 1;
+    c.tile = narrow.rows;
+    c.split = narrow.split;
+  } else {
+    c.split = 1;
+    c.tile = linear_tc_width(p, sm_count, &c.tiles);
+  }
+  return c;
+}
 
 std::string launch_linear(const LinearProblem& p, const LaunchCtx& ctx, int path_option, int* path_used,
                           std::string* refused) {

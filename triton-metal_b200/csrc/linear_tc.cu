@@ -531,13 +531,18 @@ std::string launch_tile(const LinearProblem& p, const OperandLayout& lx, const O
   return std::string();
 }
 
+// Tiles of 256 rows and `width` accumulator columns.
+int64_t tile_count(const LinearProblem& p, int width) {
+  const int64_t cols = p.mode == LinearMode::Gated ? width / 2 : width;
+  return ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + cols - 1) / cols) * (p.mode == LinearMode::Pair ? 2 : 1);
+}
+
 // Clocks of a launch with tiles of 256 x `width` accumulator columns.  What an SM takes in bounds the narrower
 // ones: a k-block's products take 256, 512 and 1024 clocks at 128, 256 and 512 columns and ask for 96, 64 and 48
 // bytes a clock; measured on 8192 x 4096 x 16384, 281, 420 and 791 ns a k-block of every pair.  The widest leaves no
 // second accumulator, so part of its epilogue is not hidden under the next tile's products.
 double tile_clocks(const LinearProblem& p, int width, int sm_count) {
-  const int64_t cols = p.mode == LinearMode::Gated ? width / 2 : width;
-  const int64_t tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + cols - 1) / cols) * (p.mode == LinearMode::Pair ? 2 : 1);
+  const int64_t tiles = tile_count(p, width);
   const int64_t blocks = (p.K + BK - 1) / BK * (p.mode == LinearMode::Sum ? 2 : 1);
   const int64_t waves = (tiles + sm_count / 2 - 1) / (sm_count / 2);
   const bool light = p.act == Act::None && p.mode != LinearMode::Gated && !p.pre && !p.residual;
@@ -581,6 +586,12 @@ std::string make_operand_map(CUtensorMap* map, CUtensorMapDataType type, const v
   }
   strides[0] = (uint64_t)l.stride * 2;
   return make_tensor_map(map, type, 2, base, dims, strides, box);
+}
+
+int linear_tc_width(const LinearProblem& p, int sm_count, int64_t* tiles) {
+  const int width = tile_width(p, sm_count);
+  *tiles = tile_count(p, width);
+  return width;
 }
 
 double estimate_linear_tc(const LinearProblem& p, int sm_count) {

@@ -31,6 +31,8 @@ std::string launch_linear_narrow(const LinearProblem& p, const OperandLayout& lx
 
 // The kernel for many rows, and an estimate of its time in clocks.
 double estimate_linear_tc(const LinearProblem& p, int sm_count);
+// Accumulator columns of its tiles (128, 256 or 512) and how many tiles there are.
+int linear_tc_width(const LinearProblem& p, int sm_count, int64_t* tiles);
 // x, w (and x2, w2) both as the layouts say; fp32 is not taken.
 std::string launch_linear_tc(const LinearProblem& p, const OperandLayout& lx, const OperandLayout& lw,
                              const LaunchCtx& ctx);

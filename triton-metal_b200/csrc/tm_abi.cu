@@ -2074,6 +2074,31 @@ int64_t tmx_debug_attention_schedule(int32_t kind, int32_t bh, int32_t rows, int
   return n;
 }
 
+// Which kernel and tile a 16-bit product takes (no device needed).
+int32_t tmx_debug_linear_choice(int32_t mode, int32_t activation, int32_t pre, int32_t residual, int64_t M, int64_t N,
+                                int64_t K, int32_t x_by_k, int32_t sm_count, int64_t* out) {
+  if (mode < 0 || mode > 3 || activation < 0 || activation >= kActCount || M <= 0 || N <= 0 || K <= 0 ||
+      M > 0x7fffffff || N > 0x7fffffff || K > 0x7fffffff || sm_count <= 0 || !out) {
+    store_error(invalid_argument("tmx_debug_linear_choice needs mode 0...3, activation 0...5 and positive 32-bit extents"));
+    return -1;
+  }
+  LinearProblem p{};
+  char some = 0;                         // an operand that is there; never read
+  p.elt = Elt::BF16;
+  p.act = (Act)activation;
+  p.mode = (LinearMode)mode;
+  p.x = p.w = p.out = &some;
+  if (p.mode != LinearMode::Single) p.w2 = &some;
+  if (p.mode == LinearMode::Sum || p.mode == LinearMode::Pair) p.x2 = &some;
+  if (p.mode == LinearMode::Pair) p.out2 = &some;
+  if (pre) p.pre = &some;
+  if (residual) p.residual = &some;
+  p.M = M; p.N = N; p.K = K;
+  const TensorChoice c = tensor_choice(p, x_by_k != 0, sm_count);
+  out[0] = c.narrow; out[1] = c.tile; out[2] = c.split; out[3] = c.tiles;
+  return 0;
+}
+
 // Writes a device status record from the host, as if a kernel's bounded wait had given up.
 int32_t tmx_debug_inject_status(int32_t code, int32_t where, int32_t block, int32_t extra) {
   std::string err;

@@ -43,6 +43,7 @@ EXPORTS = {
     "tmx_matmul_gathered": (_I32, (_I64, _I64, _I64, _I64P, _I64P, _I32, _I32, _I64, _I64, _I64, _I64, _I32,
                                    ctypes.c_uint32, _I32)),
     "tmx_debug_attention_schedule": (_I64, (_I32, _I32, _I32, _I32, _I32, _I32, _I32P, _I64, _I32P, _I64P)),
+    "tmx_debug_linear_choice": (_I32, (_I32, _I32, _I32, _I32, _I64, _I64, _I64, _I32, _I32, _I64P)),
     "tmx_selftest_bounded_wait": (_I32, (_I64, _I32P)),
     "tmx_debug_inject_status": (_I32, (_I32, _I32, _I32, _I32)),
 }
@@ -237,3 +238,14 @@ def attention_schedule(kind: str, bh: int, rows: int, n_ctx: int, causal: bool, 
     used = min(ctas, n)
     lists = [[(items[2 * i], items[2 * i + 1]) for i in range(begin[c], begin[c + 1])] for c in range(used)]
     return lists, list(load)[:used]
+
+
+LINEAR_MODES = ("linear", "gated", "sum", "pair")
+
+
+def linear_choice(mode, M, N, K, activation="none", pre=False, residual=False, x_by_k=True, sm_count=148):
+    """What a 16-bit product runs on: ("few rows", rows of x a tile, split of K) or ("pairs", columns a tile, tiles)."""
+    out = (ctypes.c_int64 * 4)()
+    _ok(_lib.tmx_debug_linear_choice(LINEAR_MODES.index(mode), ACTIVATIONS.index(activation), int(pre), int(residual),
+                                     M, N, K, int(x_by_k), sm_count, out))
+    return ("few rows", out[1], out[2]) if out[0] else ("pairs", out[1], out[3])
