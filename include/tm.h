@@ -316,7 +316,8 @@ int32_t tmx_debug_inject_status(int32_t code, int32_t where, int32_t block, int3
  *
  *   linear_kernel(x, w, [bias], [residual], out, [pre], M, N, K, [stride_xm, stride_xk, stride_wk,
  *                 stride_wn, stride_om, stride_rm, stride_pm])
- *       pre = x w + bias, out = act(pre) + residual (act takes the unrounded value)
+ *       pre = x w + bias, out = act(pre) + residual (act takes the unrounded value; gelu of minus infinity is
+ *       0, its limit, while silu and gelu_tanh of it are NaN, minus infinity times 0)
  *   gated_linear_kernel(x, w_gate, w_up, out, [pre_gate], [pre_up], M, N, K, [strides as above])
  *       pre_gate = x w_gate, pre_up = x w_up, out = act(pre_gate) * pre_up
  *   linear_sum_kernel(x, w, x2, w2, out, M, N, K, [strides])       out = x w + x2 w2
