@@ -144,3 +144,36 @@ def test_gated_gradients_keep_the_layout_of_their_own_weight(calls, gate_rows, u
         assert grad.shape == weight.shape and grad.stride() == weight.stride()
     products = [c["name"] for c in calls[2:]]
     assert products == (["linear_pair_kernel"] if gate_rows == up_rows else ["linear_kernel"] * 2)
+
+
+def test_threads_that_meet_at_a_first_call_load_its_kernel_once(calls, monkeypatch, no_leaks):
+    """A second copy would stay loaded with nobody to release it."""
+    import threading
+    import time
+
+    from triton_metal import kernels
+    made, ready = [], threading.Barrier(4)
+
+    class Slow(kernels.Linear):
+        def __init__(self, *a):
+            time.sleep(0.05)
+            super().__init__(*a)
+            made.append(self)
+
+    monkeypatch.setattr(kernels, "Linear", Slow)
+    x, w, failed = zeros(8, 16), zeros(16, 24), []
+
+    def work():
+        ready.wait()
+        try:
+            functional.linear(x, w)
+        except Exception as e:      # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and len(made) == 1 and len(calls) == 4
+    functional.release()

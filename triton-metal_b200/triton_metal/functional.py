@@ -23,6 +23,7 @@ checks addresses (device, alignment, overlap) on every launch.
 
 import math
 import struct
+import threading
 
 import torch
 from torch.autograd import forward_ad
@@ -34,15 +35,16 @@ _ELEMENT = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
 _KERNELS = {}
 _RECIPES = {}
 _MOST_RECIPES = 4096
+_loading = threading.Lock()
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def release():
     """Drop the loaded kernels and recipes (they are made again on the next call)."""
-    _RECIPES.clear()
-    for kern in _KERNELS.values():
-        kern.release()
-    _KERNELS.clear()
+    with _loading:
+        _RECIPES.clear()
+        while _KERNELS:
+            _KERNELS.popitem()[1].release()
 
 
 def check():
@@ -58,7 +60,10 @@ def _kernel(cls, dtype, operands=(), activation=None, norm=None):
     key = (cls, dtype, operands, activation, norm)
     kern = _KERNELS.get(key)
     if kern is None:
-        kern = _KERNELS[key] = cls(_ELEMENT[dtype], operands, activation, norm)
+        with _loading:                  # threads that meet here load it once
+            kern = _KERNELS.get(key)
+            if kern is None:
+                kern = _KERNELS[key] = cls(_ELEMENT[dtype], operands, activation, norm)
     return kern
 
 
