@@ -117,3 +117,52 @@ def test_tiles_of_the_cta_pairs(F, case, element, layout):
 def test_tiles_of_the_few_row_kernel(F, case, element, layout):
     mode, M, N, K = case[:4]
     check_case(F, mode, M, N, K, "pre" if mode != "sum" and M % 2 else "", TYPES[element], layout)
+
+
+# ---- several host threads ---------------------------------------------------------------------------------
+
+def test_threads_on_their_own_streams(F):
+    """First calls and later ones, each thread on its own stream and operands: the results of calls made alone, and
+    every launch counted."""
+    import threading
+
+    from triton_metal import cuda
+    dtype, count, rounds = torch.bfloat16, 8, 100
+    sets = []
+    for i in range(count):
+        M, K, N = 5 + i, 64 + 8 * (i % 3), 72 + 16 * (i % 2)
+        sets.append(dict(x=normal(M, K, dtype=dtype), w=weight(K, N, dtype, "kn"), r=normal(M, N, dtype=dtype),
+                         n=normal(N, dtype=dtype), d=normal(M, N, dtype=dtype)))
+
+    def work(t):
+        out, pre = F.linear(t["x"], t["w"], t["n"], t["r"], activation="silu", pre=True)
+        total, normed, stats = F.residual_norm(out, t["r"], t["n"], scale=0.5, stats=True)
+        back = F.residual_norm_backward(t["d"], t["r"], total, stats, t["n"], t["r"], scale=0.5)
+        return [out, normed, back[0], back[2], *F.linear_backward(t["d"], t["x"], t["w"], pre, activation="silu", bias=True)]
+
+    F.release()
+    torch.cuda.synchronize()
+    got, failed, gate = [[] for _ in sets], [], threading.Barrier(count)
+    before = cuda.launch_count()
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                gate.wait()
+                for _ in range(rounds):
+                    got[i] = work(sets[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:      # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(count)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    made = cuda.launch_count() - before
+    start, alone = cuda.launch_count(), [work(t) for t in sets]
+    assert made == rounds * (cuda.launch_count() - start)
+    for a, b in zip(got, alone):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))

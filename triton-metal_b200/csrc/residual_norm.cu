@@ -828,14 +828,15 @@ std::string launch_sized(const NormProblem& p, const LaunchCtx& ctx, bool backwa
     const bool branch = p.gate || p.post_weight;
     auto kernel = branch ? residual_norm_bwd_kernel<T, VEC, THREADS, PACKS, true>
                          : residual_norm_bwd_kernel<T, VEC, THREADS, PACKS, false>;
-    static int resident[2] = {0, 0};       // blocks of this kernel an SM holds
-    if (!resident[branch]) {
+    static std::atomic<int> known[2];      // blocks of this kernel an SM holds
+    int resident = known[branch].load(std::memory_order_relaxed);
+    if (!resident) {
       int n = 0;
       if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, BLOCK, 0) != cudaSuccess || n < 1) n = 1;
-      resident[branch] = n;
+      known[branch].store(resident = n, std::memory_order_relaxed);
     }
     // (no rows: one block, whose sums are zero)
-    const int64_t grid = std::min<int64_t>(std::max<int64_t>(blocks, 1), (int64_t)ctx.sm_count * resident[branch]);
+    const int64_t grid = std::min<int64_t>(std::max<int64_t>(blocks, 1), (int64_t)ctx.sm_count * resident);
     const int64_t groups = grid * ROWS;
     void* outs[kMaxColumnSums] = {};
     const int sets = sum_outputs(p, outs);

@@ -73,7 +73,7 @@ struct LibraryObj : Object {
 struct KernelObj : Object {
   KernelDesc desc;
   int path_option = 0;   // 0 auto, 1 SIMT, 2 tcgen05 required
-  int last_path = 0;
+  std::atomic<int> last_path{0};
   // Entry point of a binary image (null for the library's own kernels): its name, the size of
   // every parameter as the image declares them, and the image itself, kept loaded.
   cudaKernel_t binary = nullptr;
@@ -198,7 +198,7 @@ struct Device {
   // capability probe
   bool probed = false;
   std::string unusable;      // empty when usable
-  int64_t launches = 0;
+  std::atomic<int64_t> launches{0};      // (callers may be threads)
   unsigned int* gather_counter = nullptr;   // device word: CTAs of a gathered GEMM that are done
 };
 
@@ -884,6 +884,8 @@ bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
   if (k.binary) return enqueue_binary(k, gx, gy, gz, threads, kinds, values, argc, repeats, err);
   Decoded d;
   if (!decode_args(k, kinds, values, argc, d, err)) return false;
+  // held from the first event of a buffer's order to the note of the launch
+  std::unique_lock<std::recursive_mutex> order(g_dev.order_lock, std::defer_lock);
   struct NoteOnExit {
     Decoded& d;
     bool armed = false;
@@ -918,6 +920,7 @@ bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
       return false;
     }
   }
+  order.lock();
   // a buffer whose read-back may still be in flight must not be overwritten under it
   for (auto& kv : d.buffers) {
     if (kv.second && kv.second->read_async_since_write) {
@@ -1663,7 +1666,9 @@ int32_t tmx_launch_on(int64_t kernel, void* stream, int64_t gx, int64_t gy, int6
   SetUpDuringCapture relaxed;           // a kernel's first launch loads it
   LaunchCtx ctx = launch_ctx();
   ctx.stream = (cudaStream_t)stream;
+  std::unique_lock<std::recursive_mutex> order(g_dev.order_lock, std::defer_lock);
   if (stream == (void*)g_dev.stream) {
+    order.lock();
     prefetch_exposed(d);
     for (auto& kv : d.buffers) {
       if (kv.second->read_async_since_write) {

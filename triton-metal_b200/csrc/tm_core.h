@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <string>
 #include <vector>
@@ -164,7 +165,7 @@ struct LaunchCtx {
   cudaStream_t stream;
   int sm_count;
   DeviceStatus* status;   // device pointer
-  int64_t* launches;      // incremented by each launcher per kernel launched
+  std::atomic<int64_t>* launches;   // incremented by each launcher per kernel launched
 };
 
 // Launchers.  Return nullptr on success or a static/owned error string.
