@@ -256,6 +256,20 @@ bool ensure_device(std::string& err) {
   return true;
 }
 
+// Puts the calling thread's current device back where it was.
+struct KeepDevice {
+  int device = -1;
+  KeepDevice() {
+    if (cudaGetDevice(&device) != cudaSuccess) {
+      cudaGetLastError();
+      device = -1;
+    }
+  }
+  ~KeepDevice() {
+    if (device >= 0 && g_dev.ok && device != g_dev.ordinal) cudaSetDevice(device);
+  }
+};
+
 // The calling thread must have the library's device current before any CUDA call.
 bool bind_device(std::string& err) {
   if (!ensure_device(err)) return false;
@@ -1514,6 +1528,7 @@ int32_t tmx_set_device(int32_t ordinal) {
 }
 
 int32_t tmx_get_device(void) {
+  KeepDevice current;                   // asking is not using
   std::string err;
   if (!ensure_device(err)) { store_error(err); return -1; }
   return g_dev.ordinal;
@@ -1631,17 +1646,9 @@ int32_t tmx_launch_on(int64_t kernel, void* stream, int64_t gx, int64_t gy, int6
   if (threads <= 0 || threads > 1024) return fail(invalid_argument("threadsPerThreadgroup must be 1...1024"));
   FeedForwardPlan plan;
   if (!plan_feed_forward(*k, o, gx, gy, plan, err)) return fail(err);
+  KeepDevice current;                   // (the first use of the library binds its device)
   if (!ensure_device(err)) return fail(err);
-  // the caller's current device is left as it was
-  struct Restore {
-    int device = -1;
-    ~Restore() { if (device >= 0) cudaSetDevice(device); }
-  } restore;
-  int current = -1;
-  if (cudaGetDevice(&current) == cudaSuccess && current != g_dev.ordinal) {
-    restore.device = current;
-    cudaSetDevice(g_dev.ordinal);
-  }
+  if (current.device != g_dev.ordinal) cudaSetDevice(g_dev.ordinal);
   static std::atomic<bool> usable{false};       // the probe's answer does not change
   if (!usable.load(std::memory_order_relaxed)) {
     const std::string& why = unusable_reason();
