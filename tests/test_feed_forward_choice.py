@@ -35,3 +35,22 @@ def test_refusals():
             cuda.linear_choice(*bad)
     assert cuda._lib.tmx_debug_linear_choice(4, 0, 0, 0, 1, 1, 1, 1, 148, None) == -1
     assert "mode 0...3" in _core.last_error()
+
+
+def test_a_grid_whose_extent_passes_64_bits_covers_everything():
+    """2^60 programs of 128 rows are not 0 rows: the operands are looked at, and found too short."""
+    import ctypes
+
+    from triton_metal import kernels
+    for cls, scalars in ((kernels.Linear, (8, 16, 32, 32, 1, 16, 1, 16, 16, 16)),
+                         (kernels.ResidualNorm, (8, 16, _core.float_bits(1.0), _core.float_bits(1e-6), 16))):
+        kern = cls("bf16")
+        try:
+            n = len(kern.names)
+            values = (ctypes.c_int64 * n)(0x10000000, 0x20000000, 0x30000000, *scalars)
+            lengths = (ctypes.c_int64 * n)(64, 64, 64)
+            for gx, gy in ((1 << 60, 1), (1 << 57, 1), (1, 1 << 57)):
+                assert cuda._lib.tmx_launch_on(kern.handle, 0, gx, gy, 1, 128, kern._kinds, values, lengths, n) == -1
+                assert "beyond its" in _core.last_error()
+        finally:
+            kern.release()

@@ -463,6 +463,12 @@ bool check_int32(int64_t v, const char* name, std::string& err) {
   return true;
 }
 
+// What `programs` blocks of `block` cover of an extent (all of it where the kernel has no block shape).
+int64_t covered(int64_t extent, int64_t programs, int64_t block) {
+  if (block <= 0 || programs >= extent / block + (extent % block != 0)) return extent;
+  return programs * block;
+}
+
 int64_t get_int(const Decoded& d, Role r, int64_t fallback) {
   auto it = d.ints.find((int)r);
   return it == d.ints.end() ? fallback : it->second;
@@ -738,8 +744,8 @@ bool plan_feed_forward(const KernelObj& k, const Operands& o, int64_t gx, int64_
         !number(Role::StrideCm, N, "stride_om", p.som) || !number(Role::StrideRm, N, "stride_rm", p.srm) ||
         !number(Role::StridePm, N, "stride_pm", p.spm))
       return false;
-    if (desc.block_m > 0) M = std::min<int64_t>(M, gx * (int64_t)desc.block_m);
-    if (desc.block_n > 0) N = std::min<int64_t>(N, gy * (int64_t)desc.block_n);
+    M = covered(M, gx, desc.block_m);
+    N = covered(N, gy, desc.block_n);
     p.M = M; p.N = N; p.K = K;
     if (!check_int32(M, "M", err) || !check_int32(N, "N", err) || !check_int32(K, "K", err)) return false;
     if (M == 0 || N == 0) return true;
@@ -767,8 +773,8 @@ bool plan_feed_forward(const KernelObj& k, const Operands& o, int64_t gx, int64_
         !number(Role::StrideCm, N, "stride_dout", p.s_dout) || !number(Role::StridePm, N, "stride_pre", p.s_pre) ||
         !number(Role::StrideRm, N, "stride_dz", p.s_dz))
       return false;
-    if (desc.block_m > 0) M = std::min<int64_t>(M, gx * (int64_t)desc.block_m);
-    if (desc.block_n > 0) N = std::min<int64_t>(N, gy * (int64_t)desc.block_n);
+    M = covered(M, gx, desc.block_m);
+    N = covered(N, gy, desc.block_n);
     p.M = M; p.N = N;
     if (!check_int32(M, "M", err) || !check_int32(N, "N", err)) return false;
     if (N == 0) return true;
@@ -799,7 +805,7 @@ bool plan_feed_forward(const KernelObj& k, const Operands& o, int64_t gx, int64_
     if (!number(Role::M, 0, "M", p.M) || !number(Role::N, 0, "D", p.D) ||
         !number(Role::StrideAm, p.D, "stride_row", p.stride))
       return false;
-    if (desc.block_m > 0) p.M = std::min<int64_t>(p.M, gx * (int64_t)desc.block_m);
+    p.M = covered(p.M, gx, desc.block_m);
     if (!check_int32(p.M, "M", err)) return false;
     if (p.D > kNormMaxColumns) {
       err = invalid_argument(std::string(kernel_entry_name(desc.id)) + " takes rows of at most " +
@@ -996,7 +1002,7 @@ bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
       if (!check_extent(*in0, {{p.rows, p.stride_in}, {p.cols, 1}}, 4, "the input", err)) return false;
       if (!check_extent(*outb, {{p.rows, p.stride_out}, {p.cols, 1}}, 4, "the output", err)) return false;
     } else {
-      p.limit = std::min<int64_t>(get_int(d, Role::Count, 0), gx * block);
+      p.limit = block > 0 ? covered(get_int(d, Role::Count, 0), gx, block) : 0;
       if (p.limit <= 0) return true;
       if (!check_extent(*in0, {{p.limit, 1}}, 4, "the first input", err)) return false;
       if (in1 && !check_extent(*in1, {{p.limit, 1}}, 4, "the second input", err)) return false;
@@ -1027,8 +1033,8 @@ bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
         !nonneg(p.scm, "stride_cm") || !nonneg(p.scn, "stride_cn"))
       return false;
     // Programs beyond the grid were never dispatched: their tiles stay untouched.
-    if (desc.block_m > 0) M = std::min<int64_t>(M, gx * (int64_t)desc.block_m);
-    if (desc.block_n > 0) N = std::min<int64_t>(N, gy * (int64_t)desc.block_n);
+    M = covered(M, gx, desc.block_m);
+    N = covered(N, gy, desc.block_n);
     p.M = M; p.N = N; p.K = K;
     BufferObj *A = buf(Role::A), *B = buf(Role::B), *C = buf(Role::C);
     if (!A || !B || !C || (sae && !buf(Role::BiasVec))) {
@@ -1084,7 +1090,7 @@ bool enqueue(KernelObj& k, int64_t gx, int64_t gy, int64_t gz, int64_t threads,
   }
   int block_rows = desc.id == KernelId::AttnBwdDkdv ? desc.block_n : desc.block_m;
   p.rows = p.n_ctx;
-  if (block_rows > 0) p.rows = std::min<int64_t>(p.n_ctx, gx * (int64_t)block_rows);
+  if (block_rows > 0) p.rows = covered(p.n_ctx, gx, block_rows);
   if (p.n_ctx == 0 || p.rows == 0) return true;
   if (!check_int32(p.n_ctx, "n_ctx", err) || !check_int32(p.bh, "grid_y (batch*heads)", err)) return false;
   auto data = [&](Role r, const char* what, const void** slot) {
