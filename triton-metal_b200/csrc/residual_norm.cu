@@ -18,7 +18,10 @@
 // block, which keeps it in registers between the passes (statistics, second statistics, result), so
 // the variance is a true second pass over the centred values and costs no memory traffic.  The
 // backward kernel walks its rows with the column sums in registers and leaves one partial row per
-// warp or block in scratch memory for a second, ordered summation.
+// warp or block in scratch memory for a second, ordered summation.  The widest rows do not fit:
+// the backward pass of more than 8192 columns (of more than 4096 where a gate or post norm adds its sums
+// and the row is not streamed) keeps part of a row in local memory, 0.3 to 2.1 KB a thread by the
+// compiler's report; that is traffic between the passes, through L1, which the narrower rows do not have.
 
 #include "ffn_math.cuh"
 #include "sm100_ptx.cuh"
@@ -881,7 +884,6 @@ std::string launch_typed(const NormProblem& p, const LaunchCtx& ctx, bool backwa
       if (packets <= 2048) return launch_stream<T, 512, 4>(p, ctx, backward);
     }
     if (packets <= 32) return launch_sized<T, VEC, 32, 1>(p, ctx, backward);
-    if (packets <= 64) return launch_sized<T, VEC, 32, 2>(p, ctx, backward);
     if (packets <= 2048) return launch_sized<T, VEC, 512, 4>(p, ctx, backward);
     if constexpr (VEC == 4) return launch_sized<T, VEC, 512, 8>(p, ctx, backward);
   }
