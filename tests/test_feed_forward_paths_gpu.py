@@ -166,3 +166,36 @@ def test_threads_on_their_own_streams(F):
     assert made == rounds * (cuda.launch_count() - start)
     for a, b in zip(got, alone):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+# ---- what earlier work leaves behind ------------------------------------------------------------------------
+
+LEFTOVERS = [(1, 64, 64), (3, 17, 5), (16, 256, 640), (77, 520, 264), (129, 136, 1000), (300, 1025, 515), (513, 320, 1032),
+             (40, 1023, 65)]
+
+
+@pytest.mark.parametrize("shape", LEFTOVERS, ids=str)
+@pytest.mark.parametrize("element", ["bf16", "f16", "f32"])
+def test_leftovers_in_memory_do_not_reach_a_result(F, element, shape):
+    """The same call before and after one on NaN throughout, which leaves NaN in the scratch memory, the temporaries,
+    the outputs' memory, shared memory and TMEM that the next call is given."""
+    M, K, N = shape
+    dtype = TYPES[element]
+
+    def call(t):
+        out = [F.linear(t["x"], t["w"], t["b"], t["d"], activation="gelu"), *F.linear_backward(t["d"], t["x"], t["w"], t["z"],
+                                                                                             activation="silu", bias=True),
+               *F.gated_linear(t["x"], t["w"], t["v"], save=True),
+               *F.gated_linear_backward(t["d"], t["x"], t["w"], t["v"], t["z"], t["u"])]
+        total, normed, stats = F.residual_norm(t["x"], t["y"], t["n"], kind="layer", post_weight=t["n"], stats=True)
+        back = F.residual_norm_backward(t["y"], t["x"], total, stats, t["n"], t["y"], post_weight=t["n"], kind="layer", bias=True)
+        return [v for v in out + [total, normed, stats, *back] if v is not None]
+
+    t = dict(x=normal(M, K, dtype=dtype), y=normal(M, K, dtype=dtype), n=normal(K, dtype=dtype), b=normal(N, dtype=dtype),
+             w=weight(K, N, dtype, "kn"), v=weight(K, N, dtype, "nk"),
+             **{k: normal(M, N, dtype=dtype) for k in "dzu"})
+    first = [v.clone() for v in call(t)]
+    assert all(torch.isfinite(v).all() for v in first)
+    for _ in range(3):
+        call({k: torch.full_like(v, float("nan")) for k, v in t.items()})
+        assert all(torch.equal(a, b) for a, b in zip(first, call(t)))
