@@ -199,3 +199,160 @@ def test_leftovers_in_memory_do_not_reach_a_result(F, element, shape):
     for _ in range(3):
         call({k: torch.full_like(v, float("nan")) for k, v in t.items()})
         assert all(torch.equal(a, b) for a, b in zip(first, call(t)))
+
+
+# ---- in place ----------------------------------------------------------------------------------------------
+
+def launch(cls, operands, scalars, element, activation=None, norm=None):
+    """A kernel class on torch tensors by operand name (None is left out), on the current stream."""
+    present = {k: v for k, v in operands.items() if v is not None}
+    kern = cls(element, tuple(n for n in cls.OPTIONAL if n in present), activation, norm)
+    try:
+        tensors = [present[n] for n in kern.pointers]
+        kern.launch_tensors(torch.cuda.current_stream().cuda_stream, [t.data_ptr() for t in tensors],
+                            [t.numel() * t.element_size() for t in tensors], scalars)
+        torch.cuda.synchronize()
+    finally:
+        kern.release()
+
+
+IN_PLACE = [(1, 8), (7, 96), (70, 33), (300, 1024), (130, 4104), (40, 1023)]
+
+
+@pytest.mark.parametrize("element", ["bf16", "f32"])
+@pytest.mark.parametrize("shape", IN_PLACE, ids=str)
+def test_in_place_activation_gradients(F, element, shape):
+    from triton_metal import kernels
+    M, N = shape
+    dtype = TYPES[element]
+    d, z, u = (normal(M, N, dtype=dtype) for _ in range(3))
+    scalars = (M, N, N, N, N)
+    want, sums = torch.empty_like(d), torch.empty_like(d[0])
+    launch(kernels.ActivationBackward, dict(dout=d, pre=z, dz=want, dbias=sums), scalars, element, "gelu")
+    for which in (0, 1):
+        t, got = [d.clone(), z.clone()], torch.empty_like(sums)
+        launch(kernels.ActivationBackward, dict(dout=t[0], pre=t[1], dz=t[which], dbias=got), scalars, element, "gelu")
+        assert torch.equal(t[which], want) and torch.equal(got, sums)
+        assert torch.equal(t[1 - which], (z, d)[which])
+    dg, du = torch.empty_like(d), torch.empty_like(d)
+    launch(kernels.GatedActivationBackward, dict(dout=d, pre_gate=z, pre_up=u, dgate=dg, dup=du), scalars, element, "silu")
+    for a in range(3):
+        for b in range(3):
+            if a == b:
+                continue
+            t = [d.clone(), z.clone(), u.clone()]
+            launch(kernels.GatedActivationBackward, dict(dout=t[0], pre_gate=t[1], pre_up=t[2], dgate=t[a], dup=t[b]), scalars,
+                   element, "silu")
+            assert torch.equal(t[a], dg) and torch.equal(t[b], du)
+
+
+@pytest.mark.parametrize("element", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("shape", IN_PLACE + [(333, 2048), (20, 8200)], ids=str)
+def test_in_place_norm_gradients(F, element, kind, shape):
+    from triton_metal import _core, kernels
+    M, D = shape
+    dtype = TYPES[element]
+    dn, ds, s, y = (normal(M, D, dtype=dtype) for _ in range(4))
+    w, g, p = (normal(D, dtype=dtype, std=0.2, mean=1.0) for _ in range(3))
+    stats = torch.rand(M, 4, device="cuda") + 0.5
+    scalars = (M, D, _core.float_bits(0.75), D)
+    names = ("dnormed", "dsum", "block")
+
+    def run(dresidual, dblock, gate, post, **t):
+        sums = [torch.empty_like(w) for _ in range(2)]
+        launch(kernels.ResidualNormBackward,
+               dict(sum=s, stats=stats, weight=w, gate=gate, post_weight=post, dresidual=dresidual, dblock=dblock,
+                    dweight=sums[0], dbias=sums[1], **t), scalars, element, None, kind)
+        return sums
+
+    for gate, post in ((None, None), (g, None), (g, p)):
+        fresh = dict(zip(names, (dn, ds, y)))
+        dr, db = torch.empty_like(s), torch.empty_like(s)
+        want = run(dr, db, gate, post, **fresh)
+        for a in ("dnormed", "dsum"):
+            for b in names:
+                if a == b:
+                    continue
+                t = {k: v.clone() for k, v in fresh.items()}
+                got = run(t[a], t[b], gate, post, **t)
+                assert torch.equal(t[a], dr) and torch.equal(t[b], db), (a, b)
+                assert all(torch.equal(i, j) for i, j in zip(got, want)), (a, b)
+
+
+@pytest.mark.parametrize("element", ["bf16", "f16", "f32"])
+def test_in_place_residual_of_every_kernel(F, element):
+    dtype = TYPES[element]
+    for M, K, N in ((1, 4096, 264), (5, 64, 72), (300, 256, 264), (130, 65, 33), (9486, 136, 792), (1034, 72, 7464), (20, 2, 8)):
+        x, w, r = normal(M, K, dtype=dtype), weight(K, N, dtype, "kn"), normal(M, N, dtype=dtype)
+        want = F.linear(x, w, None, r, activation="relu")
+        assert F.linear(x, w, None, r, activation="relu", out=r) is r and torch.equal(r, want)
+
+
+# ---- operands the documentation allows ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("element", ["bf16", "f32"])
+def test_overlapping_rows_and_shared_operands(F, element):
+    """Windows of one signal as rows, one tensor as several operands."""
+    dtype = TYPES[element]
+    signal = normal(5000, dtype=dtype)
+    for K, hop in ((64, 8), (64, 24), (128, 1), (40, 3), (256, 16)):
+        x = signal.unfold(0, K, hop)                      # rows hop elements apart
+        w = weight(K, 72, dtype, "nk")
+        for rows in (x, x[:9], x[:1]):
+            assert torch.equal(F.linear(rows, w), F.linear(rows.contiguous(), w))
+        d = normal(x.shape[0], 72, dtype=dtype)
+        for a, b in zip(F.linear_backward(d, x, w), F.linear_backward(d, x.contiguous(), w)):
+            assert a is b is None or torch.equal(a, b)
+    for M, K, N in ((7, 64, 72), (140, 65, 33), (300, 128, 264)):
+        x, w, d = normal(M, K, dtype=dtype), weight(K, N, dtype, "nk"), normal(M, N, dtype=dtype)
+        assert torch.equal(F.gated_linear(x, w, w), F.gated_linear(x, w, w.clone()))
+        got, want = F.gated_linear_backward(d, x, w, w, d, d), F.gated_linear_backward(d, x, w, w.clone(), d.clone(), d.clone())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        n = normal(K, dtype=dtype)
+        got = F.residual_norm(x, x, n, n, n, n, stats=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, F.residual_norm(x, x.clone(), n.clone(), n.clone(), n, n, stats=True)))
+        got = F.residual_norm_backward(x, x, x, got[2], n, x, n, n, bias=True)
+        want = F.residual_norm_backward(x, x.clone(), x.clone(), F.residual_norm(x, x, n, n, n, n, stats=True)[2], n, x.clone(),
+                                        n.clone(), n.clone(), bias=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("element", ["bf16", "f16", "f32"])
+def test_extents_of_zero(F, element):
+    dtype = TYPES[element]
+    new = lambda *s: normal(*s, dtype=dtype)  # noqa: E731
+    for M, K, N in ((0, 16, 24), (5, 0, 24), (5, 16, 0), (0, 0, 0), (1, 0, 1)):
+        x, w, d, b = new(M, K), new(K, N), new(M, N), new(N)
+        out, pre = F.linear(x, w, b, d, activation="sigmoid", pre=True)
+        assert torch.equal(pre, b.expand(M, N)) or K
+        if not K:
+            error = (out.double() - (torch.sigmoid(b.double()) + d.double())).abs()
+            assert not error.numel() or float(error.max()) <= 8 * half(dtype)
+        dx, dw, db = F.linear_backward(d, x, w, d, activation="silu", bias=True)
+        assert dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape
+        assert not (dw != 0).any() and (N or not (dx != 0).any()) and (M or not (db != 0).any())
+        h, g, u = F.gated_linear(x, w, w, save=True)
+        assert h.shape == (M, N) and (K or not ((h != 0) | (g != 0) | (u != 0)).any())
+        dx, dwg, dwu = F.gated_linear_backward(d, x, w, w, g, u)
+        assert not ((dwg != 0) | (dwu != 0)).any() and (N or not (dx != 0).any())
+    total, normed, stats = F.residual_norm(new(0, 64), new(0, 64), new(64), stats=True)
+    back = F.residual_norm_backward(normed, total, total, stats, new(64), total, new(64), new(64), bias=True)
+    assert total.shape == normed.shape == (0, 64) and stats.shape == (0, 4)
+    assert all(not (v != 0).any() for v in back)
+
+
+@pytest.mark.parametrize("element", ["bf16", "f32"])
+def test_one_row_without_a_batch_dimension(F, element):
+    dtype = TYPES[element]
+    x, w, n, d = normal(264, dtype=dtype), weight(264, 72, dtype, "kn"), normal(264, dtype=dtype), normal(72, dtype=dtype)
+    one = lambda t: t.unsqueeze(0)  # noqa: E731
+    assert torch.equal(one(F.linear(x, w, None, d)), F.linear(one(x), w, None, one(d)))
+    for a, b in zip(F.linear_backward(d, x, w), F.linear_backward(one(d), one(x), w)):
+        assert a is b is None or torch.equal(a, b.view(a.shape))
+    assert torch.equal(one(F.gated_linear(x, w, w)), F.gated_linear(one(x), w, w))
+    s, m, st = F.residual_norm(x, x, n, stats=True)
+    wanted = F.residual_norm(one(x), one(x), n, stats=True)
+    assert s.shape == m.shape == x.shape and all(torch.equal(a.view(b.shape), b) for a, b in zip((s, m, st), wanted))
+    got = F.residual_norm_backward(m, s, s, st, n, x)
+    assert got[0].shape == got[1].shape == x.shape
