@@ -356,3 +356,64 @@ def test_one_row_without_a_batch_dimension(F, element):
     assert s.shape == m.shape == x.shape and all(torch.equal(a.view(b.shape), b) for a, b in zip((s, m, st), wanted))
     got = F.residual_norm_backward(m, s, s, st, n, x)
     assert got[0].shape == got[1].shape == x.shape
+
+
+# ---- operands of more than 2^31 elements --------------------------------------------------------------------
+
+FAR = 5                                    # rows at the far end that hold something
+
+
+def far(M, N, dtype):
+    """Zeros, but for the first and the last few rows."""
+    t = torch.zeros(M, N, device="cuda", dtype=dtype)
+    assert t.numel() > 1 << 31
+    for rows in (t[:FAR], t[-FAR:]):
+        rows.copy_(normal(FAR, N, dtype=dtype))
+    return t
+
+
+def test_far_rows_of_the_norms_and_activation_gradients(F):
+    dtype, M, D = torch.bfloat16, 140000, 16384
+    w, g, p = (normal(D, dtype=dtype, std=0.1, mean=1.0) for _ in range(3))
+    r, y = far(M, D, dtype), far(M, D, dtype)
+    ends = lambda *ts: [torch.cat([t[:FAR], t[-FAR:]]) for t in ts]  # noqa: E731
+    total, normed, stats = F.residual_norm(r, y, w, w, g, p, kind="layer", stats=True)
+    want = F.residual_norm(*ends(r, y), w, w, g, p, kind="layer", stats=True)
+    assert all(torch.equal(a, b) for a, b in zip(ends(total, normed, stats), want))
+    del normed, r
+    dn = far(M, D, dtype)
+    got = F.residual_norm_backward(dn, None, total, stats, w, y, g, p, kind="layer")[:2]
+    back = F.residual_norm_backward(*ends(dn), None, *ends(total, stats), w, *ends(y), g, p, kind="layer")
+    assert all(torch.equal(a, b) for a, b in zip(ends(*got), back))
+    del got, total
+    one = weight(8, D, dtype, "kn")
+    x = torch.zeros(M, 8, device="cuda", dtype=dtype)
+    dx, _, db = F.linear_backward(dn, x, one, y, activation="silu", bias=True)       # dz of 2^31 elements and more
+    few = F.linear_backward(*ends(dn, x), one, *ends(y), activation="silu", bias=True)
+    scale = float(few[0].double().abs().max())
+    assert float((ends(dx)[0].double() - few[0].double()).abs().max()) < 2 * half(dtype) * scale
+    assert not (dx[FAR:-FAR] != 0).any()
+    assert float((db.double() - few[2].double()).abs().max()) < 2 * half(dtype) * float(few[2].double().abs().max())
+
+
+@pytest.mark.parametrize("element", ["bf16", "f32"])
+def test_far_columns_of_weights_and_rows_of_outputs(F, element):
+    """Weights of more than 2^31 elements (aligned, and at an odd pitch, which are copied first), then outputs."""
+    dtype = TYPES[element]
+    for K, N in ((70000, 32768),) + (((70001, 32765),) if element == "bf16" else ()):
+        w = torch.zeros(K, N, device="cuda", dtype=dtype)
+        w[-64:].copy_(normal(64, N, dtype=dtype, std=0.125))
+        for M in (3, 200):
+            x = normal(M, K, dtype=dtype)
+            z, slack = product64(x[:, -64:], w[-64:])
+            check(F.linear(x, w), z, slack)
+        del w
+    for K, N in ((64, 32768), (2, 32769)):
+        M = 70000
+        x, w = normal(M, K, dtype=dtype), weight(K, N, dtype, "kn")
+        out = F.linear(x, w)
+        for rows in (slice(0, 9), slice(M - 9, M)):
+            z, slack = product64(x[rows], w)
+            check(out[rows], z, slack)
+        del out
+    torch.cuda.empty_cache()
