@@ -335,7 +335,8 @@ int32_t tmx_debug_inject_status(int32_t code, int32_t where, int32_t block, int3
  *                            [dresidual], [dblock], [dweight], [dbias], [dgate], [dpost_weight], scale,
  *                            M, D, [stride_row])
  * Option "path" on the products: 0 picks the kernel, 1 forces the CUDA cores, 2 requires the tensor cores and refuses
- * what they do not take (fp32, whose products are formed in fp32; K = 0).
+ * what they do not take (fp32, whose products are formed in fp32; K = 0).  On the CUDA cores a product has at most
+ * 8388480 columns, a gated one 4194240.
  * The grid has the meaning of the IR's block shape, as for matmul_kernel: rows beyond grid_x * BLOCK_M
  * (and, for the products and activation gradients, columns beyond grid_y * BLOCK_N) are left as they
  * are.  Rows of the norms have at most 16384 columns.  Gradients of a linear layer: dx = dz w^T and

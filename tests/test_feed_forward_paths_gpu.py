@@ -417,3 +417,17 @@ def test_far_columns_of_weights_and_rows_of_outputs(F, element):
             check(out[rows], z, slack)
         del out
     torch.cuda.empty_cache()
+
+
+def test_the_widest_products_on_the_cuda_cores(F):
+    """The last size that is taken is right to its last column, and the refusal of the next names the limit."""
+    for columns, call in ((8388480, lambda x, w: F.linear(x, w)), (4194240, lambda x, w: F.gated_linear(x, w, w, activation="none"))):
+        x, w = normal(2, 3, dtype=torch.float32), normal(3, columns + 1, dtype=torch.float32)
+        z, slack = product64(x, w[:, :columns])
+        got = call(x, w[:, :columns])
+        if columns == 8388480:
+            check(got, z, slack)
+        else:
+            check(got, z * z, slack * (2 * z.abs() + slack) + 2.0 ** -23 * z * z)
+        with pytest.raises(RuntimeError, match=f"more than {columns} columns"):
+            call(x, w)

@@ -404,7 +404,7 @@ std::string launch_tile(const LinearProblem& p, const LaunchCtx& ctx) {
   const int cols = GATED ? TN / 2 : TN;
   const int64_t gx = (p.M + TM - 1) / TM, gy = (p.N + cols - 1) / cols;
   const int64_t gz = p.mode == LinearMode::Pair ? 2 : 1;
-  if (gy > 65535) return "more than 65535 column blocks (4194240 columns)";
+  if (gy > 65535) return "more than " + std::to_string(65535 * cols) + " columns";
   if (gx > 0x0fffffff) return "too many rows";
   const int64_t steps = (p.K + TK - 1) / TK * (p.mode == LinearMode::Sum ? 2 : 1);
   f.split = split_of(gx * gy * gz, steps, ctx.sm_count);

@@ -1,7 +1,9 @@
 // The feed-forward matrix products on the CUDA cores: every element type, any strides and
-// alignment, extents from zero up.  fp32 operands always come here: their products are formed in
-// fp32 (the tensor core's tf32 accumulator truncates, which costs an order of magnitude of error),
-// so the bound is the FMA pipe - 2 x 128 lanes x 148 SMs x 1.9 GHz, 72 TFLOP/s.
+// alignment, extents from zero up.  What comes here is what the other kernels do not take: K = 0,
+// 16-bit products of K < 33 with an operand that the TMA cannot fetch (or with no memory for its
+// aligned copy, or when the CUDA cores are asked for), and fp32 operands without a contiguous
+// dimension (the others have linear_f32.cu).  The bound is the FMA pipe - 2 x 128 lanes x 148 SMs x
+// 1.9 GHz, 72 TFLOP/s.
 //
 // Tile 128 x 128 x 16, 256 threads, 8 x 8 outputs each as two 4-wide halves 64 rows / columns
 // apart (so that the 16-byte shared-memory reads of a quarter-warp touch distinct banks), the next
@@ -137,7 +139,7 @@ std::string launch_typed(const LinearProblem& p, const LaunchCtx& ctx) {
   const bool gated = p.mode == LinearMode::Gated;
   const int cols = gated ? TN / 2 : TN;
   const int64_t gx = (p.M + TM - 1) / TM, gy = (p.N + cols - 1) / cols;
-  if (gy > 65535) return "more than 65535 column blocks (4194240 columns)";
+  if (gy > 65535) return "more than " + std::to_string(65535 * cols) + " columns";
   const dim3 grid((unsigned)gx, (unsigned)gy, p.mode == LinearMode::Pair ? 2 : 1);
   if (gated) linear_simt_kernel<T, true><<<grid, 256, 0, ctx.stream>>>(p);
   else linear_simt_kernel<T, false><<<grid, 256, 0, ctx.stream>>>(p);
