@@ -431,3 +431,35 @@ def test_the_widest_products_on_the_cuda_cores(F):
             check(got, z * z, slack * (2 * z.abs() + slack) + 2.0 ** -23 * z * z)
         with pytest.raises(RuntimeError, match=f"more than {columns} columns"):
             call(x, w)
+
+
+def test_products_that_take_longer_than_a_wait_may(F):
+    """Sums so long that a tile takes about as long as the bounded waits' second, or longer: nothing gives up."""
+    dtype, at = torch.bfloat16, [0, 1, 77, 1 << 28, (1 << 29) - 3]
+    # few rows: one row, one column, K of almost 2^31
+    K = (1 << 31) - 600
+    x, w = torch.zeros(1, K, device="cuda", dtype=dtype), torch.zeros(K, 1, device="cuda", dtype=dtype)
+    far_at = torch.tensor(at + [K - 1, K // 2], device="cuda")
+    x[0, far_at], w[far_at, 0] = normal(far_at.numel(), dtype=dtype), normal(far_at.numel(), dtype=dtype)
+    z, slack = product64(x[:, far_at], w[far_at])
+    check(F.linear(x, w), z, slack)
+    nothing_gave_up(F)
+    del x, w
+    # the CTA pairs: the gradient of a 2 x 2 weight over 2^29 rows
+    M = 1 << 29
+    x, d, w = torch.zeros(M, 2, device="cuda", dtype=dtype), torch.zeros(M, 2, device="cuda", dtype=dtype), weight(2, 2, dtype, "kn")
+    rows = torch.tensor(at, device="cuda")
+    x[rows], d[rows] = normal(len(at), 2, dtype=dtype), normal(len(at), 2, dtype=dtype)
+    dx, dw, _ = F.linear_backward(d, x, w)
+    nothing_gave_up(F)
+    z, slack = product64(x[rows].t(), d[rows])
+    check(dw, z, slack)
+    z, slack = product64(d[rows], w.t())
+    check(dx[rows], z, slack)
+    del x, d, dx
+    torch.cuda.empty_cache()
+
+
+def nothing_gave_up(F):
+    torch.cuda.synchronize()
+    F.check()

@@ -273,7 +273,9 @@ linear_narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ 
     // ------------------------------------------------------------ accumulator, thread = output column
     // (after a wait that gave up the sums are whatever is there, and the launch is reported as failed; by vote, so
     // that the lanes come to the warp-wide loads together whichever of them saw the barrier or gave up first)
-    mbar_wait_warp(smem_u32(&bars.acc_full), 0, wc, kEpiAccFull);
+    // The wait lasts as long as all of the CTA's products do, a few hundred clocks a k-block (4096 allowed).
+    const WaitCtx all_blocks{&bars.abort_flag, status, kWaitCycles + 4096ll * (kb1 - kb0)};
+    mbar_wait_warp(smem_u32(&bars.acc_full), 0, all_blocks, kEpiAccFull);
     tc_fence_after();
     const int quarter = warp % 4;
     const uint32_t lanes = tmem_base + ((uint32_t)(quarter * 32) << 16);

@@ -392,6 +392,8 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
     const int quarter = warp % 4, part = warp / 4;
     const uint32_t piece = smem_base + STAGES * STAGE_BYTES + warp * BOX;
     const Act act = (Act)a.act;
+    // one wait of these warps lasts as long as a tile's products do: up to 1040 clocks a k-block (4096 allowed)
+    const WaitCtx tile_wait{&bars.abort_flag, status, kWaitCycles + 4096ll * k_blocks};
     bool staged = false;                // a TMA store may still be reading the piece
     bool ok = true;
     int local = 0;
@@ -422,7 +424,7 @@ linear_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args
         const int acc = HALVES == 2 ? half : local & 1;
         const uint32_t turn = HALVES == 2 ? local & 1 : (local >> 1) & 1;
         // (the lanes leave together: one that gave up alone would be missed by the next warp-wide load)
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full[acc]), turn, wc, kEpiAccFull))) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.acc_full[acc]), turn, tile_wait, kEpiAccFull))) { ok = false; break; }
         tc_fence_after();
         // (the allocation is ordered before the products that filled the accumulator)
         const uint32_t lanes = *(volatile uint32_t*)&bars.tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
