@@ -323,7 +323,7 @@ int32_t tmx_debug_inject_status(int32_t code, int32_t where, int32_t block, int3
  *   linear_sum_kernel(x, w, x2, w2, out, M, N, K, [strides])       out = x w + x2 w2
  *   linear_pair_kernel(x, w, x2, w2, out, out2, M, N, K, [strides])  out = x w, out2 = x2 w2
  *   activation_bwd_kernel(dout, [pre], [dz], [dbias], M, N, [stride_dout, stride_pre, stride_dz])
- *       dz = dout act'(pre), dbias[n] = sum over m of the unrounded dz
+ *       dz = dout act'(pre), dbias[n] = sum over m of the unrounded dz (relu'(0) = 0)
  *   gated_activation_bwd_kernel(dout, pre_gate, pre_up, dgate, dup, M, N, [strides as above])
  *       dgate = dout pre_up act'(pre_gate), dup = dout act(pre_gate)
  *   residual_norm_kernel(residual, [block], weight, [bias], [gate], [post_weight], [sum], normed,

@@ -121,8 +121,9 @@ __global__ void __launch_bounds__(CX * RY) activation_bwd_kernel(const ActBwdPro
 template <typename T, int VEC>
 std::string launch_vec(const ActBwdProblem& p, const LaunchCtx& ctx) {
   const int64_t gx = (p.N + CX * VEC - 1) / (CX * VEC);
-  // Each block has at least 32 rows; up to 64 one block takes them all and no second launch is needed.  With column sums about eight blocks per SM, so that the sums stay cheap;
-  // without, more (8192 x 4096 gated: 62 us with eight, 53 with 24).
+  // Each block has at least 32 rows; up to 64 one block takes them all and no second launch is needed.  With
+  // column sums about eight blocks per SM, so that the sums stay cheap; without, more (8192 x 4096 gated: 62 us
+  // with eight, 53 with 24).
   int64_t gy = std::max<int64_t>(1, (int64_t)ctx.sm_count * (p.gated ? 24 : 8) / gx);
   gy = p.M <= 64 && !p.gated ? 1 : std::min(gy, std::max<int64_t>(1, (p.M + 31) / 32));
   gy = std::min<int64_t>(gy, 65535);

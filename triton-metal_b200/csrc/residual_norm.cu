@@ -12,7 +12,7 @@
 //   with h_y = dt post_weight;  dweight = sum dnormed s^;  dbias = sum dnormed;
 //   dgate = sum ds t;  dpost = sum dt y^       ([mean(...)]: layer norm only; sums over the rows)
 //
-// Aligned rows of 1024 bytes and more are streamed: persistent blocks fetch their next rows by bulk
+// Aligned rows of more than 512 bytes are streamed: persistent blocks fetch their next rows by bulk
 // copies into a shared-memory ring while they work on the current one, and keep the weights in
 // registers.  HBM-bound: each [M, D] operand crosses the memory bus once.  A row belongs to one warp or one
 // block, which keeps it in registers between the passes (statistics, second statistics, result), so

@@ -15,6 +15,11 @@ what the forward pass returned and return new tensors (a weight's gradient in th
 weight).  No graph is recorded, so an operand that requires grad is refused while grad mode is on (and one
 that carries a forward-mode tangent always).  The reference has no counterpart.
 
+Operands that the kernels cannot take as they lie are copied on every call: an x whose leading dimensions are
+not a fixed distance apart or whose rows are not contiguous, a vector with a stride, [rows, D] operands of the
+norms that are not dense (a column slice of a wider tensor), one of two gate and up weights in different
+layouts, and, inside the library, 16-bit operands of a product that are not aligned to 16 bytes.
+
 Every call goes through a recipe: the checks of shapes, types and strides, the temporaries, and the
 launches with everything but the addresses.  Recipes depend on the operands' metadata alone and are
 kept by it, so a repeated call pays for its allocations, its addresses and its launches; the library
