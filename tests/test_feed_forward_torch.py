@@ -177,3 +177,15 @@ def test_threads_that_meet_at_a_first_call_load_its_kernel_once(calls, monkeypat
         t.join()
     assert not failed and len(made) == 1 and len(calls) == 4
     functional.release()
+
+
+def test_a_release_during_a_first_call_leaves_no_dead_recipe(calls, monkeypatch):
+    """Another thread's release() between the load of a call's kernel and the call's end: later calls load it again."""
+    real = functional._kernel
+    monkeypatch.setattr(functional, "_kernel", lambda *a: (real(*a), functional.release())[0])
+    x, w = zeros(8, 16), zeros(16, 24)
+    with pytest.raises(StopIteration):          # (the launch that is written down finds no such kernel)
+        functional.linear(x, w)
+    monkeypatch.setattr(functional, "_kernel", real)
+    functional.linear(x, w)
+    assert len(calls) == 1

@@ -41,12 +41,14 @@ _KERNELS = {}
 _RECIPES = {}
 _MOST_RECIPES = 4096
 _loading = threading.Lock()
+_released = [0]             # how often release() has run
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def release():
     """Drop the loaded kernels and recipes (they are made again on the next call)."""
     with _loading:
+        _released[0] += 1
         _RECIPES.clear()
         while _KERNELS:
             _KERNELS.popitem()[1].release()
@@ -219,12 +221,14 @@ def _refuse_tangents(names, tensors):
             raise RuntimeError(f"{name} carries a forward-mode tangent" + _NO_GRAPH)
 
 
-def _keep(key, recipe):
-    if len(_RECIPES) >= _MOST_RECIPES:
-        _RECIPES.clear()
+def _keep(key, recipe, released):
     recipe.tensors = dict.fromkeys(recipe.tensors)       # metadata only: no operand is held
-    _RECIPES[key] = recipe
-    return recipe
+    with _loading:
+        if released != _released[0]:                     # its kernels have been dropped since
+            return
+        if len(_RECIPES) >= _MOST_RECIPES:
+            _RECIPES.clear()
+        _RECIPES[key] = recipe
 
 
 def _call(build, static, names, tensors):
@@ -239,9 +243,10 @@ def _call(build, static, names, tensors):
     except AttributeError:          # not a tensor: the recipe says which
         key = recipe = None
     if recipe is None:
+        released = _released[0]
         recipe = _Recipe(**dict(zip(names, tensors)))
         build(recipe, *static)
-        _keep(key, recipe)
+        _keep(key, recipe, released)
     return recipe.run(tensors)
 
 
