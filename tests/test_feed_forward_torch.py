@@ -189,3 +189,13 @@ def test_a_release_during_a_first_call_leaves_no_dead_recipe(calls, monkeypatch)
     monkeypatch.setattr(functional, "_kernel", real)
     functional.linear(x, w)
     assert len(calls) == 1
+
+
+def test_statistics_of_rows_without_columns_are_refused(calls):
+    """Nothing would be launched, and the statistics would be whatever their memory holds."""
+    r, w = zeros(3, 0), zeros(0)
+    total, normed = functional.residual_norm(r, r, w)
+    assert total.shape == normed.shape == (3, 0)
+    with pytest.raises(ValueError, match="rows without columns have no statistics"):
+        functional.residual_norm(r, r, w, stats=True)
+    functional.residual_norm(zeros(0, 8), None, zeros(8), stats=True)

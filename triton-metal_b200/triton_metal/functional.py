@@ -420,6 +420,8 @@ def _plan_residual_norm(r, kind, scale, eps, stats):
     passed = r.tensors["block"] is None and scale == 1.0     # sum is residual itself
     total = None if passed else r.new(shape)
     normed = r.new(shape)
+    if stats and not D:
+        raise ValueError("rows without columns have no statistics")
     rows = r.new((residual.rows, 4), torch.float32) if stats else None
     operands.update(residual=residual, block=r.rows("block", dense=True), bias=r.vector("bias", D), sum=total,
                     normed=normed, stats=rows)
